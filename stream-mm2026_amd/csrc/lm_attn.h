@@ -1,0 +1,37 @@
+// lm_attn.h -- launches of the attention kernels (lm_attn_kernel.h, lm_attn_bf16.hip, lm_attn_f16.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace lm {
+
+// A [batch, heads, positions, dim] array: elements between batches, heads and positions; dim is dense.
+struct AttnTensor {
+    void *p;
+    int64_t b, h, t;
+};
+
+struct AttnArgs {
+    AttnTensor q, k, v, o, dout, dq, dk, dv;
+    const uint8_t *key_mask;       // [batch, keys] (0: hidden), rows mask_stride apart, or null
+    int64_t mask_stride;
+    float *lse;                    // [batch, heads, rows]: log sum exp of the scaled scores
+    float *delta;                  // backward's workspace, as lse: rowsum(dout * out)
+    float *partial;                // forward's workspace where the keys are split
+    int batch, heads, key_heads, group;   // heads = key_heads * group
+    int rows, keys, dim;           // row i stands at position keys - rows + i
+    int window, sinks;             // row at p sees key j <= p if p - j < window or j < sinks
+    float scale;
+    int splits;
+};
+
+template <int DT>
+hipError_t attn_forward(const AttnArgs &a, hipStream_t stream);
+template <int DT>
+hipError_t attn_backward(const AttnArgs &a, hipStream_t stream);
+
+// How many parts the keys are split into, and the floats of workspace that takes.
+int attn_splits(const AttnArgs &a);
+int64_t attn_forward_workspace(const AttnArgs &a);
+
+}  // namespace lm

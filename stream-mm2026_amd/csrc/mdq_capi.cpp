@@ -17,16 +17,15 @@
 
 #include "../../include/stquant_hip.h"
 #include "mdq_desc.h"
+#include "mdq_error.h"
 #include "mdq_launch.h"
 #include "mdq_math.h"
 #include "mdq_convert.h"
 #include "mdq_stats.h"
 
-namespace {
+namespace mdq {
 
-using mdq::MdqDesc;
-
-thread_local std::string g_err;
+static thread_local std::string g_err;
 
 int fail(int code, const char *fmt, ...)
 {
@@ -60,6 +59,16 @@ const char *dtype_name(int dt)
     default: return "Unknown";
     }
 }
+
+}  // namespace mdq
+
+namespace {
+
+using mdq::MdqDesc;
+using mdq::dtype_name;
+using mdq::fail;
+using mdq::g_err;
+using mdq::hip_fail;
 
 // Storage dispatch of stquant_kernel.cu:430-464.  Returns the storage class or
 // -1 (message set).  packed4 needs bits == 4, uint8 m codes, empty v codes.

@@ -54,6 +54,24 @@ EXPORTED_SYMBOLS = (
 )
 
 
+# Every symbol include/stquant_lm.h declares (the transformer operators).
+LM_SYMBOLS = (
+    "stq_embedding_forward",
+    "stq_embedding_grad_workspace",
+    "stq_embedding_backward",
+    "stq_norm_residual_workspace",
+    "stq_norm_residual_forward",
+    "stq_norm_residual_backward",
+    "stq_attention_forward_workspace",
+    "stq_attention_backward_workspace",
+    "stq_attention_forward",
+    "stq_attention_backward",
+    "stq_distill_forward",
+    "stq_distill_backward",
+    "stq_lm_abi_version",
+)
+LM_ABI_VERSION = 1
+
 # STQ_ABI_VERSION of include/stquant_hip.h this package is written against
 ABI_VERSION = 4
 
@@ -153,6 +171,31 @@ def lib() -> ctypes.CDLL:
         raise RuntimeError(f"{LIB_PATH} has ABI version {L.stq_abi_version()}, this package needs "
                            f"{ABI_VERSION}: rebuild it")
     _lib = L
+    return L
+
+
+_lm_lib = None
+
+
+def lm_lib() -> ctypes.CDLL:
+    """``lib()`` with the entry points of include/stquant_lm.h bound: each takes its argument struct as packed
+    bytes, and the launching ones a stream."""
+    global _lm_lib
+    if _lm_lib is not None:
+        return _lm_lib
+    L = lib()
+    for name in LM_SYMBOLS:
+        fn = getattr(L, name)
+        if name.endswith("_workspace"):
+            fn.argtypes, fn.restype = [ctypes.c_char_p], ctypes.c_int64
+        elif name.endswith("_version"):
+            fn.argtypes, fn.restype = [], ctypes.c_int
+        else:
+            fn.argtypes, fn.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
+    if L.stq_lm_abi_version() != LM_ABI_VERSION:
+        raise RuntimeError(f"{LIB_PATH} has operator ABI version {L.stq_lm_abi_version()}, this package needs "
+                           f"{LM_ABI_VERSION}: rebuild it")
+    _lm_lib = L
     return L
 
 
