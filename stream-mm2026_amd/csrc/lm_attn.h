@@ -30,8 +30,24 @@ hipError_t attn_forward(const AttnArgs &a, hipStream_t stream);
 template <int DT>
 hipError_t attn_backward(const AttnArgs &a, hipStream_t stream);
 
-// How many parts the keys are split into, and the floats of workspace that takes.
+// How many parts the keys are split into where there are few rows, and the floats of workspace that takes.
+constexpr int MAX_SPLITS = 512;
 int attn_splits(const AttnArgs &a);
 int64_t attn_forward_workspace(const AttnArgs &a);
+
+// Where the work on the keys' gradients is cut: blocks of 128 keys, and for the first `sink_blocks` of
+// them `far` more shares of `step` positions each, which lie behind the window of the block's keys.
+struct DkvSplit {
+    int blocks, sink_blocks, far, step;
+    // The partial sums of share f (0: the blocks' own): dk and dv of the sinks.
+    __host__ __device__ float *sums(const AttnArgs &a, int head, int f) const
+    {
+        return a.partial + ((int64_t)head * (far + 1) + f) * 2 * a.sinks * a.dim;
+    }
+};
+DkvSplit dkv_split(const AttnArgs &a);
+// The floats of workspace: delta, then the partial sums.
+int64_t attn_backward_delta(const AttnArgs &a);
+int64_t attn_backward_workspace(const AttnArgs &a);
 
 }  // namespace lm

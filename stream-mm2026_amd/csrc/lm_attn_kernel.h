@@ -16,8 +16,9 @@
 // rows of one column.  Softmax statistics then belong to lanes (a column is a row of the attention):
 // maximum and sum need one exchange between the wave's halves.
 //
-// LDS tiles are row major, 16-byte pieces XOR-ed with their row so that both the row reads (16
-// lanes, 16 rows, one piece) and the transposing reads (4 rows x 2 pieces) fall on different banks.
+// LDS tiles are row major with 32 bytes between rows: eight lanes of a row read (8 rows, one 16-byte
+// piece each) and sixteen of a transposing read (4 rows x 32 bytes) then fall on different banks, and
+// every address is a lane's base plus a constant.
 #pragma once
 #include "lm_attn.h"
 #include "lm_common.h"
@@ -53,29 +54,24 @@ __device__ __forceinline__ f32x16 zero16()
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
-// A tile of rows of HD 16-bit elements in LDS.
+// A tile of rows of HD 16-bit elements in LDS, 32 bytes between rows.
 template <int HD>
 struct Tile {
-    static constexpr int PIECES = HD / 8, ROW = HD * 2;
-    static __device__ __forceinline__ int turn(int row)
-    {
-        return HD == 128 ? ((row & 7) << 1) | ((row >> 3) & 1) : (row & 6) | ((row >> 3) & 1);
-    }
-    static __device__ __forceinline__ int at(int row, int piece) { return row * ROW + ((piece ^ turn(row)) << 4); }
+    static constexpr int ROW = HD * 2 + 32;
 
     // A operand, its k along the elements: row `row` + lane & 31, elements 16 c + 8 half ...
     static __device__ __forceinline__ u32x4 rows(const char *t, int row, int c, int lane)
     {
-        return *(const u32x4 *)(t + at(row + (lane & 31), 2 * c + (lane >> 5)));
+        return *(const u32x4 *)(t + ((lane & 31) * ROW + (lane >> 5) * 16) + (row * ROW + c * 32));
     }
     // A operand, its k along the rows: element 32 d + lane & 31 of the 16 rows from `row`, in the
     // order of a result's registers
     static __device__ __forceinline__ u32x4 columns(const char *t, int row, int d, int lane)
     {
         typedef __attribute__((address_space(3))) s16x4 *lds4;
-        const int i = lane & 15, r = row + 4 * (lane >> 5) + (i >> 2), piece = 4 * d + ((lane >> 3) & 2) + ((i >> 1) & 1);
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(t + at(r, piece) + (i & 1) * 8));
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(t + at(r + 8, piece) + (i & 1) * 8));
+        const char *p = t + ((4 * (lane >> 5) + ((lane >> 2) & 3)) * ROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8) + (row * ROW + d * 64);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 8 * ROW));
         const u32x2 u = __builtin_bit_cast(u32x2, x), w = __builtin_bit_cast(u32x2, y);
         return u32x4{u[0], u[1], w[0], w[1]};
     }
@@ -119,55 +115,88 @@ struct KeyTiles {
     __device__ __forceinline__ int key(int i) const { return (i < sink_tiles ? i : first + i - sink_tiles) * TILE; }
 };
 
-// THREADS threads bring a tile of rows from memory to LDS by way of registers: load(), then store()
-// once the tile's last readers are done.  Rows outside [0, rows) and elements from dim on are zero,
-// and so are the rows that `hidden` names: what lies there (a masked key may hold anything) must not
-// meet a weight of zero.
-template <int HD, int THREADS>
+// A buffer descriptor over the memory from p on: 32-bit byte offsets, and an offset of 2^31 and more
+// reads zeros without touching memory.
+constexpr uint32_t NOWHERE = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_from(const void *p)
+{
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, NOWHERE, 0x00027000);
+}
+
+// THREADS threads bring a tile of ROWS rows from memory to LDS by way of registers: load(), then
+// store() once the tile's last readers are done.  A piece at NOWHERE is zero: rows that are not
+// there, elements from dim on, and masked keys, which may hold anything and must not meet a weight
+// of zero.
+template <int HD, int THREADS, int ROWS>
 struct Stage {
-    static constexpr int N = TILE * HD / 8 / THREADS;
+    static constexpr int N = ROWS * HD / 8 / THREADS, STEP = THREADS * 8 / HD;      // rows between a thread's pieces
     u32x4 v[N];
 
-    template <typename Address, typename Valid>
-    __device__ __forceinline__ void load(Address address, Valid valid, int dim)
+    static __device__ __forceinline__ int row() { return threadIdx.x / (HD / 8); }
+    static __device__ __forceinline__ int piece() { return threadIdx.x % (HD / 8); }
+    template <typename Offset>
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t from, Offset offset)
     {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int e = i * THREADS + threadIdx.x, row = e / (HD / 8), d = e % (HD / 8) * 8;
-            v[i] = u32x4{0, 0, 0, 0};
-            if (d < dim && valid(row)) v[i] = *(const u32x4 *)(address(row) + d);
-        }
+        for (int i = 0; i < N; i++)
+            v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, offset(i), 0, 0));
     }
     __device__ __forceinline__ void store(char *tile) const
     {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int e = i * THREADS + threadIdx.x, row = e / (HD / 8), piece = e % (HD / 8);
-            *(u32x4 *)(tile + Tile<HD>::at(row, piece)) = v[i];
-        }
+        for (int i = 0; i < N; i++) *(u32x4 *)(tile + (row() + i * STEP) * Tile<HD>::ROW + piece() * 16) = v[i];
     }
 };
 
-// The bits of the keys [key, key + 64) that the mask shows.
-__device__ __forceinline__ uint64_t shown(const AttnArgs &a, int b, int key)
-{
-    if (!a.key_mask) return ~0ull;
-    const int j = key + (threadIdx.x & 63);
-    return __ballot(j < a.keys && a.key_mask[b * a.mask_stride + j] != 0);
-}
+// A tile of 64 keys: its rows of k and v, and which of them are shown.
+template <int HD, int THREADS>
+struct KeyStage {
+    Stage<HD, THREADS, TILE> k, v;
+    uint64_t see;
+
+    __device__ __forceinline__ void load(const AttnArgs &a, int b, int hk, int key)
+    {
+        using S = Stage<HD, THREADS, TILE>;
+        see = ~0ull;
+        if (a.key_mask) {
+            const int j = key + (threadIdx.x & 63);
+            see = __ballot(j < a.keys && a.key_mask[b * a.mask_stride + j] != 0);
+        }
+        const int left = a.keys - key;
+        const uint64_t there = see & (left < TILE ? (1ull << left) - 1 : ~0ull);
+        const auto kr = buffer_from((const uint16_t *)a.k.p + b * a.k.b + hk * a.k.h + key * a.k.t);
+        const auto vr = buffer_from((const uint16_t *)a.v.p + b * a.v.b + hk * a.v.h + key * a.v.t);
+        const int row = S::row(), d = S::piece() * 8;
+        const uint32_t kt = (uint32_t)a.k.t * 2, vt = (uint32_t)a.v.t * 2;
+        const uint32_t ko = d < a.dim ? row * kt + d * 2 : NOWHERE, vo = d < a.dim ? row * vt + d * 2 : NOWHERE;
+        if (there == ~0ull) {
+            k.load(kr, [&](int i) { return ko + i * S::STEP * kt; });
+            v.load(vr, [&](int i) { return vo + i * S::STEP * vt; });
+        } else {
+            auto shown = [&](int i) { return there >> (row + i * S::STEP) & 1; };
+            k.load(kr, [&](int i) { return shown(i) ? ko + i * S::STEP * kt : NOWHERE; });
+            v.load(vr, [&](int i) { return shown(i) ? vo + i * S::STEP * vt : NOWHERE; });
+        }
+    }
+    __device__ __forceinline__ void store(char *ktile, char *vtile) const
+    {
+        k.store(ktile);
+        v.store(vtile);
+    }
+};
 
 __device__ __forceinline__ const uint16_t *at(const AttnTensor &t, int b, int h) { return (const uint16_t *)t.p + b * t.b + h * t.h; }
 
 // ---------------------------------------------------------------- forward
 // WAVES x 32 rows; the keys in tiles of 64, or the share of them that blockIdx.z takes.
 template <int DT, int HD, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void attn_fwd_kernel(AttnArgs a)
+__global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void attn_fwd_kernel(AttnArgs a)
 {
     constexpr int C = HD / 16, ND = HD / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2][TILE * HD * 2];
+    __shared__ __attribute__((aligned(16))) char lds[2][TILE * Tile<HD>::ROW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = blockIdx.y / a.key_heads, hk = blockIdx.y % a.key_heads;
-    const int total = a.rows * a.group, r0 = blockIdx.x * WAVES * 32, row = r0 + wave * 32 + (lane & 31);
+    const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
+    const int total = a.rows * a.group, r0 = (gridDim.y - 1 - blockIdx.y) * WAVES * 32, row = r0 + wave * 32 + (lane & 31);
     const Sight sight = {a.window, a.sinks};
     const int before = a.keys - a.rows;
     const int rr = min(row, total - 1), t = rr / a.group, head = hk * a.group + rr % a.group, pos = before + t;
@@ -193,25 +222,15 @@ __global__ __launch_bounds__(WAVES * 64) void attn_fwd_kernel(AttnArgs a)
     for (int d = 0; d < ND; d++) o[d] = zero16();
     float m = -__builtin_inff(), l = 0.0f;         // in units of log2; l of this lane's keys alone
     const float c2 = a.scale * LOG2E;
-    const uint16_t *kp = at(a.k, b, hk), *vp = at(a.v, b, hk);
-    Stage<HD, WAVES * 64> ks, vs;
-    uint64_t next_shown = 0;
-    auto fetch = [&](int it) {
-        const int key = tiles.key(it);
-        next_shown = shown(a, b, key);
-        auto valid = [&](int r) { return key + r < a.keys && (next_shown >> r & 1); };
-        ks.load([&](int r) { return kp + (int64_t)(key + r) * a.k.t; }, valid, a.dim);
-        vs.load([&](int r) { return vp + (int64_t)(key + r) * a.v.t; }, valid, a.dim);
-    };
-    if (it0 < it1) fetch(it0);
+    KeyStage<HD, WAVES * 64> next;
+    if (it0 < it1) next.load(a, b, hk, tiles.key(it0));
     for (int it = it0; it < it1; it++) {
         const int key = tiles.key(it);
-        const uint64_t see = next_shown;
+        const uint64_t see = next.see;
         __syncthreads();
-        ks.store(lds[0]);
-        vs.store(lds[1]);
+        next.store(lds[0], lds[1]);
         __syncthreads();
-        if (it + 1 < it1) fetch(it + 1);
+        if (it + 1 < it1) next.load(a, b, hk, tiles.key(it + 1));
         if (see == 0 || sight.none(pa, pb, key, key + TILE - 1)) continue;
 
         f32x16 s[2] = {zero16(), zero16()};
@@ -265,8 +284,8 @@ __global__ __launch_bounds__(WAVES * 64) void attn_fwd_kernel(AttnArgs a)
     if (!real) return;
     if (a.splits > 1) {
         // unnormalised sums, their maximum and weight, for the join
-        const int64_t at_row = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * total + row;
-        float *po = a.partial + at_row * a.dim, *ml = a.partial + (int64_t)a.splits * gridDim.y * total * a.dim + at_row * 2;
+        const int64_t at_row = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * total + row;
+        float *po = a.partial + at_row * a.dim, *ml = a.partial + (int64_t)a.splits * gridDim.x * total * a.dim + at_row * 2;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -293,33 +312,51 @@ __global__ __launch_bounds__(WAVES * 64) void attn_fwd_kernel(AttnArgs a)
     if (lane < 32) a.lse[((int64_t)b * a.heads + head) * a.rows + t] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * LN2;
 }
 
-// Joins the parts of the keys: one wave a row, a lane for 2 elements.
+// Joins the parts of the keys: a workgroup a row, its waves every fourth part, a lane 2 elements.
 template <int DT>
-__global__ __launch_bounds__(64) void attn_join_kernel(AttnArgs a)
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a)
 {
-    const int total = a.rows * a.group, row = blockIdx.x, lane = threadIdx.x;
-    const int b = blockIdx.y / a.key_heads, hk = blockIdx.y % a.key_heads;
-    const int64_t rows = (int64_t)gridDim.y * total, at_row = (int64_t)blockIdx.y * total + row;
+    __shared__ float weight[MAX_SPLITS], sums[4][128], buf[2][4];
+    const int total = a.rows * a.group, row = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
+    const int64_t rows = (int64_t)gridDim.x * total, at_row = (int64_t)blockIdx.x * total + row;
     const float *ml = a.partial + a.splits * rows * a.dim;
-    float m = -__builtin_inff();
-    for (int z = 0; z < a.splits; z++) m = fmaxf(m, ml[(z * rows + at_row) * 2]);
+    const int z = threadIdx.x;                       // MAX_SPLITS = 2 x 256 parts at most
+    f32x2 p[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        p[i] = z + 256 * i < a.splits ? *(const f32x2 *)(ml + ((z + 256 * i) * rows + at_row) * 2) : f32x2{-__builtin_inff(), 0.0f};
+    const float m = group_reduce<4>(fmaxf(p[0][0], p[1][0]), [](float x, float y) { return fmaxf(x, y); }, buf[0]);
     const float ref = m == -__builtin_inff() ? 0.0f : m;
-    float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    const int e = 2 * lane;
-    for (int z = 0; z < a.splits; z++) {
-        const float w = exp2_hw(ml[(z * rows + at_row) * 2] - ref);
-        l += w * ml[(z * rows + at_row) * 2 + 1];
-        if (e < a.dim) {
-            const f32x2 v = *(const f32x2 *)(a.partial + (z * rows + at_row) * a.dim + e);
-            o0 += w * v[0];
-            o1 += w * v[1];
-        }
+    float l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float w = exp2_hw(p[i][0] - ref);
+        weight[z + 256 * i] = w;
+        l += w * p[i][1];
     }
+    l = group_reduce<4>(l, Add(), buf[1]);           // (its barrier also shows the weights)
+    float o0 = 0.0f, o1 = 0.0f;
+    const int e = 2 * lane;
+    if (e < a.dim) {
+#pragma unroll 8
+        for (int i = wave; i < a.splits; i += 4) {
+            const f32x2 v = *(const f32x2 *)(a.partial + (i * rows + at_row) * a.dim + e);
+            o0 += weight[i] * v[0];
+            o1 += weight[i] * v[1];
+        }
+        sums[wave][e] = o0;
+        sums[wave][e + 1] = o1;
+    }
+    __syncthreads();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int t = row / a.group, head = hk * a.group + row % a.group;
-    uint16_t *po = (uint16_t *)at(a.o, b, head) + t * a.o.t;
-    if (e < a.dim) *(uint32_t *)(po + e) = pack2<DT>(o0 * inv, o1 * inv);
-    if (lane == 0) a.lse[((int64_t)b * a.heads + head) * a.rows + t] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * LN2;
+    if (wave == 0 && e < a.dim) {
+        o0 = sums[0][e] + sums[1][e] + sums[2][e] + sums[3][e];
+        o1 = sums[0][e + 1] + sums[1][e + 1] + sums[2][e + 1] + sums[3][e + 1];
+        *(uint32_t *)((uint16_t *)at(a.o, b, head) + t * a.o.t + e) = pack2<DT>(o0 * inv, o1 * inv);
+    }
+    if (threadIdx.x == 0) a.lse[((int64_t)b * a.heads + head) * a.rows + t] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * LN2;
 }
 
 // ---------------------------------------------------------------- backward
@@ -350,13 +387,13 @@ __device__ __forceinline__ float score_gradient(float p, float dp, float delta) 
 
 // dq of WAVES x 32 rows: the forward pass's walk over the keys.
 template <int DT, int HD, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void attn_dq_kernel(AttnArgs a)
+__global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a)
 {
     constexpr int C = HD / 16, ND = HD / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2][TILE * HD * 2];
+    __shared__ __attribute__((aligned(16))) char lds[2][TILE * Tile<HD>::ROW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = blockIdx.y / a.key_heads, hk = blockIdx.y % a.key_heads;
-    const int total = a.rows * a.group, r0 = blockIdx.x * WAVES * 32, row = r0 + wave * 32 + (lane & 31);
+    const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
+    const int total = a.rows * a.group, r0 = (gridDim.y - 1 - blockIdx.y) * WAVES * 32, row = r0 + wave * 32 + (lane & 31);
     const Sight sight = {a.window, a.sinks};
     const int before = a.keys - a.rows;
     const int rr = min(row, total - 1), t = rr / a.group, head = hk * a.group + rr % a.group, pos = before + t;
@@ -387,25 +424,15 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dq_kernel(AttnArgs a)
 #pragma unroll
     for (int d = 0; d < ND; d++) dq[d] = zero16();
     const float c2 = a.scale * LOG2E;
-    const uint16_t *kp = at(a.k, b, hk), *vp = at(a.v, b, hk);
-    Stage<HD, WAVES * 64> ks, vs;
-    uint64_t next_shown = 0;
-    auto fetch = [&](int it) {
-        const int key = tiles.key(it);
-        next_shown = shown(a, b, key);
-        auto valid = [&](int r) { return key + r < a.keys && (next_shown >> r & 1); };
-        ks.load([&](int r) { return kp + (int64_t)(key + r) * a.k.t; }, valid, a.dim);
-        vs.load([&](int r) { return vp + (int64_t)(key + r) * a.v.t; }, valid, a.dim);
-    };
-    fetch(0);
+    KeyStage<HD, WAVES * 64> next;
+    next.load(a, b, hk, tiles.key(0));
     for (int it = 0; it < tiles.count; it++) {
         const int key = tiles.key(it);
-        const uint64_t see = next_shown;
+        const uint64_t see = next.see;
         __syncthreads();
-        ks.store(lds[0]);
-        vs.store(lds[1]);
+        next.store(lds[0], lds[1]);
         __syncthreads();
-        if (it + 1 < tiles.count) fetch(it + 1);
+        if (it + 1 < tiles.count) next.load(a, b, hk, tiles.key(it + 1));
         if (see == 0 || sight.none(pa, pb, key, key + TILE - 1)) continue;
         const bool whole = see == ~0ull && sight.all(pa, pb, key, key + TILE - 1);
 #pragma unroll
@@ -448,17 +475,23 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dq_kernel(AttnArgs a)
         }
 }
 
-// dk and dv of WAVES x 32 keys: over the rows that see any of them, 64 at a time.
+// dk and dv of WAVES x 32 keys: over the rows that see any of them, 32 at a time.  A workgroup takes the
+// positions whose window holds a key of its block; those behind that, which see the sinks alone, go to
+// workgroups of their own (DkvSplit), whose sums are fp32 partial results.
 template <int DT, int HD, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(AttnArgs a)
+__global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dkv_kernel(AttnArgs a, DkvSplit cut)
 {
     constexpr int C = HD / 16, ND = HD / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2][TILE * HD * 2];
-    __shared__ __attribute__((aligned(16))) float lse_s[TILE], delta_s[TILE];
-    __shared__ __attribute__((aligned(16))) int pos_s[TILE];
+    using S = Stage<HD, WAVES * 64, 32>;
+    __shared__ __attribute__((aligned(16))) char lds[2][32 * Tile<HD>::ROW];
+    __shared__ __attribute__((aligned(16))) float lse_s[32], delta_s[32];
+    __shared__ __attribute__((aligned(16))) int pos_s[32];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = blockIdx.y / a.key_heads, hk = blockIdx.y % a.key_heads;
-    const int k0 = blockIdx.x * WAVES * 32, ka = k0 + wave * 32, key = ka + (lane & 31);
+    const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
+    // blockIdx.y: the blocks of keys, then the sinks' far positions
+    const int far = (int)blockIdx.y < cut.blocks ? -1 : ((int)blockIdx.y - cut.blocks) % cut.far;
+    const int block = far < 0 ? blockIdx.y : (blockIdx.y - cut.blocks) / cut.far;
+    const int k0 = block * WAVES * 32, ka = k0 + wave * 32, key = ka + (lane & 31);
     const Sight sight = {a.window, a.sinks};
     const int before = a.keys - a.rows, total = a.rows * a.group;
     const bool real = key < a.keys;
@@ -479,84 +512,112 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(AttnArgs a)
 #pragma unroll
     for (int d = 0; d < ND; d++) dk[d] = dv[d] = zero16();
     const float c2 = a.scale * LOG2E;
-    // the positions that see a key of this workgroup
+    // the positions that see a key of this workgroup: [p0, p1)
     const int k1 = min(a.keys, k0 + WAVES * 32) - 1;
-    const int t0 = max(0, k0 - before);
-    const int t1 = k0 < a.sinks ? a.rows - 1 : (int)min((int64_t)a.rows - 1, (int64_t)k1 + a.window - 1 - before);
-    const int first = t0 * a.group, last = (t1 + 1) * a.group;
-    Stage<HD, WAVES * 64> qs, gs;
+    const int near = min(a.keys, k1 + a.window);
+    int p0 = max(k0, before), p1 = near;
+    if (far >= 0) {
+        p0 = max(near + far * cut.step, before);
+        p1 = min(a.keys, near + (far + 1) * cut.step);
+    } else if (k0 < a.sinks && cut.far == 0) p1 = a.keys;
+    const int first = (p0 - before) * a.group, last = (p1 - before) * a.group;      // rows
+    S qs, gs;
     float lse_r = 0.0f, delta_r = 0.0f;
     int pos_r = 0;
+    const float per_group = 1.0f / (float)a.group;
     auto fetch = [&](int row0) {
-        auto valid = [&](int r) { return row0 + r < last; };
-        auto head = [&](int r) { return hk * a.group + (row0 + r) % a.group; };
-        qs.load([&](int r) { return at(a.q, b, head(r)) + (row0 + r) / a.group * a.q.t; }, valid, a.dim);
-        gs.load([&](int r) { return at(a.dout, b, head(r)) + (row0 + r) / a.group * a.dout.t; }, valid, a.dim);
-        if (threadIdx.x < TILE) {
-            const int r = min(row0 + (int)threadIdx.x, total - 1);
-            const int64_t stat = ((int64_t)b * a.heads + hk * a.group + r % a.group) * a.rows + r / a.group;
+        // row0 + r is position t0 + (over + r) / group: small numbers, divided in fp32
+        const int t0 = row0 / a.group, over = row0 - t0 * a.group;
+        const auto qr = buffer_from(at(a.q, b, hk * a.group) + t0 * a.q.t), gr = buffer_from(at(a.dout, b, hk * a.group) + t0 * a.dout.t);
+        uint32_t qo[S::N], go[S::N];
+#pragma unroll
+        for (int i = 0; i < S::N; i++) {
+            const int r = S::row() + i * S::STEP, t = (int)(((float)(over + r) + 0.5f) * per_group), g = over + r - t * a.group;
+            const bool there = row0 + r < last && S::piece() * 8 < a.dim;
+            qo[i] = there ? (t * (uint32_t)a.q.t + g * (uint32_t)a.q.h + S::piece() * 8) * 2 : NOWHERE;
+            go[i] = there ? (t * (uint32_t)a.dout.t + g * (uint32_t)a.dout.h + S::piece() * 8) * 2 : NOWHERE;
+        }
+        qs.load(qr, [&](int i) { return qo[i]; });
+        gs.load(gr, [&](int i) { return go[i]; });
+        if (threadIdx.x < 32) {
+            const int r = min(row0 + (int)threadIdx.x, total - 1), t = r / a.group;
+            const int64_t stat = ((int64_t)b * a.heads + hk * a.group + r - t * a.group) * a.rows + t;
             lse_r = a.lse[stat] * LOG2E;
-            // no weight where a row sees nothing, nor behind the last row
             delta_r = a.delta[stat];
+            // no weight where a row sees nothing, nor behind the last row
             if (lse_r == -__builtin_inff() || row0 + (int)threadIdx.x >= last) {
                 lse_r = __builtin_inff();
                 delta_r = 0.0f;
             }
-            pos_r = before + r / a.group;
+            pos_r = before + t;
         }
     };
     if (first < last) fetch(first);
-    for (int row0 = first; row0 < last; row0 += TILE) {
+    for (int row0 = first; row0 < last; row0 += 32) {
         __syncthreads();
         qs.store(lds[0]);
         gs.store(lds[1]);
-        if (threadIdx.x < TILE) {
+        if (threadIdx.x < 32) {
             lse_s[threadIdx.x] = lse_r;
             delta_s[threadIdx.x] = delta_r;
             pos_s[threadIdx.x] = pos_r;
         }
         __syncthreads();
-        if (row0 + TILE < last) fetch(row0 + TILE);
+        if (row0 + 32 < last) fetch(row0 + 32);
+        const int pa = before + row0 / a.group, pb = before + min(row0 + 31, last - 1) / a.group;
+        if (sight.none(pa, pb, ka, ka + 31)) continue;
+        const bool whole = all_seen && sight.all(pa, pb, ka, ka + 31);
+        f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-            if (row0 + 32 * n >= last) continue;
-            const int pa = before + (row0 + 32 * n) / a.group, pb = before + (min(row0 + 32 * n + 31, last - 1)) / a.group;
-            if (sight.none(pa, pb, ka, ka + 31)) continue;
-            const bool whole = all_seen && sight.all(pa, pb, ka, ka + 31);
-            f32x16 s = zero16(), dp = zero16();
+        for (int c = 0; c < C; c++) {
+            s = mma<DT>(Tile<HD>::rows(lds[0], 0, c, lane), kf[c], s);
+            dp = mma<DT>(Tile<HD>::rows(lds[1], 0, c, lane), vf[c], dp);
+        }
 #pragma unroll
-            for (int c = 0; c < C; c++) {
-                s = mma<DT>(Tile<HD>::rows(lds[0], 32 * n, c, lane), kf[c], s);
-                dp = mma<DT>(Tile<HD>::rows(lds[1], 32 * n, c, lane), vf[c], dp);
-            }
+        for (int r = 0; r < 16; r += 4) {
+            const int i = result_row(r, lane);
+            const f32x4 ls = *(const f32x4 *)(lse_s + i), de = *(const f32x4 *)(delta_s + i);
+            if (whole) {
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int i = 32 * n + result_row(r, lane);
-                const f32x4 ls = *(const f32x4 *)(lse_s + i), de = *(const f32x4 *)(delta_s + i);
+                for (int k = 0; k < 4; k++) {
+                    s[r + k] = exp2_hw(__builtin_fmaf(s[r + k], c2, -ls[k]));
+                    dp[r + k] = s[r + k] * (dp[r + k] - de[k]);
+                }
+            } else {
                 const u32x4 po = *(const u32x4 *)(pos_s + i);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    float p = exp2_hw(__builtin_fmaf(s[r + k], c2, -ls[k]));
-                    if (whole) dp[r + k] = p * (dp[r + k] - de[k]);
-                    else {
-                        if (!(seen && sight.one((int)po[k], key))) p = 0.0f;
-                        dp[r + k] = score_gradient(p, dp[r + k], de[k]);
-                    }
-                    s[r + k] = p;
+                    const float p = exp2_hw(__builtin_fmaf(s[r + k], c2, -ls[k]));
+                    s[r + k] = seen && sight.one((int)po[k], key) ? p : 0.0f;
+                    dp[r + k] = score_gradient(s[r + k], dp[r + k], de[k]);
                 }
             }
+        }
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const u32x4 p = operand<DT>(s, 8 * k), ds = operand<DT>(dp, 8 * k);
+        for (int k = 0; k < 2; k++) {
+            const u32x4 p = operand<DT>(s, 8 * k), ds = operand<DT>(dp, 8 * k);
 #pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    dv[d] = mma<DT>(Tile<HD>::columns(lds[1], 32 * n + 16 * k, d, lane), p, dv[d]);
-                    dk[d] = mma<DT>(Tile<HD>::columns(lds[0], 32 * n + 16 * k, d, lane), ds, dk[d]);
-                }
+            for (int d = 0; d < ND; d++) {
+                dv[d] = mma<DT>(Tile<HD>::columns(lds[1], 16 * k, d, lane), p, dv[d]);
+                dk[d] = mma<DT>(Tile<HD>::columns(lds[0], 16 * k, d, lane), ds, dk[d]);
             }
         }
     }
     if (!real) return;
+    if (cut.far && key < a.sinks) {
+        float *part = cut.sums(a, blockIdx.x, far + 1) + key * a.dim;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int e = 32 * d + result_row(r, lane);
+                if (e >= a.dim) continue;
+                *(f32x4 *)(part + e) = f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
+                *(f32x4 *)(part + a.sinks * a.dim + e) = f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+            }
+        return;
+    }
+    if (far >= 0) return;
     uint16_t *pk = (uint16_t *)at(a.dk, b, hk) + (int64_t)key * a.dk.t, *pv = (uint16_t *)at(a.dv, b, hk) + (int64_t)key * a.dv.t;
 #pragma unroll
     for (int d = 0; d < ND; d++)
@@ -570,25 +631,44 @@ __global__ __launch_bounds__(WAVES * 64) void attn_dkv_kernel(AttnArgs a)
         }
 }
 
+// Adds the partial sums of the sinks: a thread 2 elements of one key.
+template <int DT>
+__global__ __launch_bounds__(256) void attn_sinks_kernel(AttnArgs a, DkvSplit cut)
+{
+    const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
+    const int i = blockIdx.y * 256 + threadIdx.x, key = i / (a.dim / 2), e = i % (a.dim / 2) * 2;
+    if (key >= a.sinks) return;
+    f32x2 k = {0.0f, 0.0f}, v = {0.0f, 0.0f};
+    for (int f = 0; f <= cut.far; f++) {
+        const float *part = cut.sums(a, blockIdx.x, f) + key * a.dim + e;
+        k += *(const f32x2 *)part;
+        v += *(const f32x2 *)(part + a.sinks * a.dim);
+    }
+    *(uint32_t *)((uint16_t *)at(a.dk, b, hk) + (int64_t)key * a.dk.t + e) = pack2<DT>(k[0] * a.scale, k[1] * a.scale);
+    *(uint32_t *)((uint16_t *)at(a.dv, b, hk) + (int64_t)key * a.dv.t + e) = pack2<DT>(v[0], v[1]);
+}
+
 template <int DT, int HD>
 void run_forward(const AttnArgs &a, hipStream_t stream)
 {
-    const int total = a.rows * a.group;
+    const int total = a.rows * a.group, heads = a.batch * a.key_heads;
     if (total <= 32)
-        attn_fwd_kernel<DT, HD, 1><<<dim3(1, a.batch * a.key_heads, a.splits), 64, 0, stream>>>(a);
+        attn_fwd_kernel<DT, HD, 1><<<dim3(heads, 1, a.splits), 64, 0, stream>>>(a);
     else
-        attn_fwd_kernel<DT, HD, 4><<<dim3((total + 127) / 128, a.batch * a.key_heads, a.splits), 256, 0, stream>>>(a);
-    if (a.splits > 1) attn_join_kernel<DT><<<dim3(total, a.batch * a.key_heads), 64, 0, stream>>>(a);
+        attn_fwd_kernel<DT, HD, 4><<<dim3(heads, (total + 127) / 128, a.splits), 256, 0, stream>>>(a);
+    if (a.splits > 1) attn_join_kernel<DT><<<dim3(heads, total), 256, 0, stream>>>(a);
 }
 
 template <int DT, int HD>
 void run_backward(const AttnArgs &a, hipStream_t stream)
 {
-    const int total = a.rows * a.group;
+    const int total = a.rows * a.group, heads = a.batch * a.key_heads;
     const int64_t rows = (int64_t)a.batch * a.heads * a.rows;
+    const DkvSplit cut = dkv_split(a);
     if (rows) attn_delta_kernel<DT><<<(unsigned)((rows + 31) / 32), 256, 0, stream>>>(a);
-    attn_dkv_kernel<DT, HD, 4><<<dim3((a.keys + 127) / 128, a.batch * a.key_heads), 256, 0, stream>>>(a);
-    if (rows) attn_dq_kernel<DT, HD, 4><<<dim3((total + 127) / 128, a.batch * a.key_heads), 256, 0, stream>>>(a);
+    attn_dkv_kernel<DT, HD, 4><<<dim3(heads, cut.blocks + cut.sink_blocks * cut.far), 256, 0, stream>>>(a, cut);
+    if (cut.far) attn_sinks_kernel<DT><<<dim3(heads, (a.sinks * a.dim / 2 + 255) / 256), 256, 0, stream>>>(a, cut);
+    if (rows) attn_dq_kernel<DT, HD, 4><<<dim3(heads, (total + 127) / 128), 256, 0, stream>>>(a);
 }
 
 }  // namespace

@@ -161,6 +161,8 @@ int check_tensor4(const char *name, const stq_tensor4 &t)
     CHECK(check_ptr(name, t.p, 16));
     if (t.batch_stride % 8 || t.head_stride % 8 || t.row_stride % 8)
         return fail(STQ_ERR_INVALID, "%s: strides must be multiples of 8 elements", name);
+    // a tile of 64 rows and the heads that share a key head are addressed by 31 bits of bytes
+    if (t.row_stride < 0 || t.row_stride > 1 << 22 || t.head_stride < 0) return fail(STQ_ERR_INVALID, "%s: row_stride must be 0 to 2^22, head_stride >= 0", name);
     return STQ_OK;
 }
 
@@ -175,9 +177,10 @@ int check_attention_sizes(const stq_attention *a)
     if (a->heads % a->key_heads)
         return fail(STQ_ERR_INVALID, "heads (%lld) must be a multiple of key_heads (%lld)", (long long)a->heads, (long long)a->key_heads);
     CHECK(check_size("batch * key_heads", a->batch * a->key_heads, 0, 65535));
-    CHECK(check_size("keys", a->keys, 0, 1 << 28));
+    // (a launch has at most 65535 tiles of 128 rows, or 128 keys and their shares)
+    CHECK(check_size("keys", a->keys, 0, 1 << 22));
     CHECK(check_size("rows", a->rows, 0, a->keys));
-    CHECK(check_size("rows * heads / key_heads", a->rows * (a->heads / a->key_heads), 0, 1 << 30));
+    CHECK(check_size("rows * heads / key_heads", a->rows * (a->heads / a->key_heads), 0, 1 << 22));
     CHECK(check_size("dim", a->dim, 8, 128));
     if (a->dim % 8) return fail(STQ_ERR_INVALID, "dim must be a multiple of 8, got %lld", (long long)a->dim);
     if (a->window < 0 || a->sinks < 0) return bad("window and sinks must be >= 0");
@@ -189,6 +192,9 @@ int check_attention(const stq_attention *a, bool backward)
     CHECK(check_attention_sizes(a));
     if (!(a->scale > 0.0) || !std::isfinite(a->scale)) return bad("scale must be finite and > 0");
     if (a->batch == 0 || a->keys == 0 || (a->rows == 0 && !backward)) return STQ_OK;
+    const int64_t group = a->heads / a->key_heads;
+    if (a->rows && (group * a->q.head_stride > 1 << 29 || (backward && group * a->dout.head_stride > 1 << 29)))
+        return bad("q and dout: the heads of a key head must lie within 2^29 elements");
     if (a->key_mask && a->key_mask_stride < 0) return bad("key_mask_stride must be >= 0");
     CHECK(check_tensor4("k", a->k));
     CHECK(check_tensor4("v", a->v));
@@ -370,7 +376,7 @@ int64_t stq_attention_forward_workspace(const stq_attention *a)
 int64_t stq_attention_backward_workspace(const stq_attention *a)
 {
     if (check_attention_sizes(a) != STQ_OK) return -1;
-    return 4 * a->batch * a->heads * a->rows;
+    return a->batch && a->keys ? 4 * lm::attn_backward_workspace(attn_args(a)) : 0;
 }
 
 int stq_attention_forward(const stq_attention *a, void *stream)
@@ -394,7 +400,8 @@ int stq_attention_backward(const stq_attention *a, void *stream)
     if (need) CHECK(check_ptr("workspace", a->workspace, 16));
     if (a->workspace_bytes < need)
         return fail(STQ_ERR_INVALID, "workspace needs %lld bytes, got %lld", (long long)need, (long long)a->workspace_bytes);
-    const lm::AttnArgs o = attn_args(a);
+    lm::AttnArgs o = attn_args(a);
+    o.partial = o.delta + lm::attn_backward_delta(o);
     return done(a->dtype == STQ_BFLOAT16 ? lm::attn_backward<lm::DT_BF16>(o, (hipStream_t)stream) : lm::attn_backward<lm::DT_F16>(o, (hipStream_t)stream),
                 "attention backward");
 }
