@@ -32,6 +32,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int FEW = 8;                          // parts of the keys that one wave joins
 constexpr int TILE = 64;                       // keys (backward for the keys: rows) of an LDS tile
 
 template <int DT>
@@ -91,7 +92,7 @@ __device__ __forceinline__ int result_row(int r, int lane) { return 8 * (r >> 2)
 // What a row at position p sees, and what a block of rows sees of a block of keys.
 struct Sight {
     int window, sinks;
-    __device__ __forceinline__ bool one(int p, int j) const { return j <= p && (p - j < window || j < sinks); }
+    __device__ __forceinline__ bool one(int p, int j) const { return (j <= p) & ((p - j < window) | (j < sinks)); }
     __device__ __forceinline__ bool none(int pa, int pb, int ka, int kb) const
     {
         return ka > pb || (pa - kb >= window && ka >= sinks);
@@ -123,6 +124,27 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_from(const void *p)
     return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, NOWHERE, 0x00027000);
 }
 
+// Which of a lane's 16 results its row at position p sees: bit r for key + result_row(r), of the 32
+// keys from `key` on that `shown` shows.
+__device__ __forceinline__ uint32_t visible16(const Sight &sight, int p, int key, uint32_t shown, int lane)
+{
+    uint32_t bits = 0;
+    shown >>= 4 * (lane >> 5);
+    key += 4 * (lane >> 5);
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        const int j = 8 * (r >> 2) + (r & 3);
+        bits |= (uint32_t)(sight.one(p, key + j) & (bool)(shown >> j & 1)) << r;
+    }
+    return bits;
+}
+
+__device__ __forceinline__ void hide(f32x16 &s, uint32_t visible)
+{
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] = (visible >> r & 1) ? s[r] : -__builtin_inff();
+}
+
 // THREADS threads bring a tile of ROWS rows from memory to LDS by way of registers: load(), then
 // store() once the tile's last readers are done.  A piece at NOWHERE is zero: rows that are not
 // there, elements from dim on, and masked keys, which may hold anything and must not meet a weight
@@ -151,37 +173,42 @@ struct Stage {
 // A tile of 64 keys: its rows of k and v, and which of them are shown.
 template <int HD, int THREADS>
 struct KeyStage {
-    Stage<HD, THREADS, TILE> k, v;
-    uint64_t see;
+    using S = Stage<HD, THREADS, TILE>;
+    S k, v;
+    uint32_t mask;                 // the mask's byte of key `lane`; looked at in store(), when it has come
 
     __device__ __forceinline__ void load(const AttnArgs &a, int b, int hk, int key)
     {
-        using S = Stage<HD, THREADS, TILE>;
-        see = ~0ull;
-        if (a.key_mask) {
-            const int j = key + (threadIdx.x & 63);
-            see = __ballot(j < a.keys && a.key_mask[b * a.mask_stride + j] != 0);
-        }
         const int left = a.keys - key;
-        const uint64_t there = see & (left < TILE ? (1ull << left) - 1 : ~0ull);
+        if (a.key_mask) {
+            const int j = threadIdx.x & 63;
+            mask = j < left ? a.key_mask[b * a.mask_stride + key + j] : 0;
+        }
         const auto kr = buffer_from((const uint16_t *)a.k.p + b * a.k.b + hk * a.k.h + key * a.k.t);
         const auto vr = buffer_from((const uint16_t *)a.v.p + b * a.v.b + hk * a.v.h + key * a.v.t);
         const int row = S::row(), d = S::piece() * 8;
         const uint32_t kt = (uint32_t)a.k.t * 2, vt = (uint32_t)a.v.t * 2;
         const uint32_t ko = d < a.dim ? row * kt + d * 2 : NOWHERE, vo = d < a.dim ? row * vt + d * 2 : NOWHERE;
-        if (there == ~0ull) {
+        if (left >= TILE) {
             k.load(kr, [&](int i) { return ko + i * S::STEP * kt; });
             v.load(vr, [&](int i) { return vo + i * S::STEP * vt; });
         } else {
-            auto shown = [&](int i) { return there >> (row + i * S::STEP) & 1; };
-            k.load(kr, [&](int i) { return shown(i) ? ko + i * S::STEP * kt : NOWHERE; });
-            v.load(vr, [&](int i) { return shown(i) ? vo + i * S::STEP * vt : NOWHERE; });
+            k.load(kr, [&](int i) { return row + i * S::STEP < left ? ko + i * S::STEP * kt : NOWHERE; });
+            v.load(vr, [&](int i) { return row + i * S::STEP < left ? vo + i * S::STEP * vt : NOWHERE; });
         }
     }
-    __device__ __forceinline__ void store(char *ktile, char *vtile) const
+    // Returns which keys are shown; the hidden ones' rows are zero.
+    __device__ __forceinline__ uint64_t store(const AttnArgs &a, char *ktile, char *vtile)
     {
+        const uint64_t see = a.key_mask ? __ballot(mask != 0) : ~0ull;
+        if (see != ~0ull) {
+#pragma unroll
+            for (int i = 0; i < S::N; i++)
+                if (!(see >> (S::row() + i * S::STEP) & 1)) k.v[i] = v.v[i] = u32x4{0, 0, 0, 0};
+        }
         k.store(ktile);
         v.store(vtile);
+        return see;
     }
 };
 
@@ -194,7 +221,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
 {
     constexpr int C = HD / 16, ND = HD / 32;
     __shared__ __attribute__((aligned(16))) char lds[2][TILE * Tile<HD>::ROW];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
     const int total = a.rows * a.group, r0 = (gridDim.y - 1 - blockIdx.y) * WAVES * 32, row = r0 + wave * 32 + (lane & 31);
     const Sight sight = {a.window, a.sinks};
@@ -226,9 +253,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
     if (it0 < it1) next.load(a, b, hk, tiles.key(it0));
     for (int it = it0; it < it1; it++) {
         const int key = tiles.key(it);
-        const uint64_t see = next.see;
         __syncthreads();
-        next.store(lds[0], lds[1]);
+        const uint64_t see = next.store(a, lds[0], lds[1]);
         __syncthreads();
         if (it + 1 < it1) next.load(a, b, hk, tiles.key(it + 1));
         if (see == 0 || sight.none(pa, pb, key, key + TILE - 1)) continue;
@@ -240,12 +266,10 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
             for (int n = 0; n < 2; n++) s[n] = mma<DT>(Tile<HD>::rows(lds[0], 32 * n, c, lane), q[c], s[n]);
         if (see != ~0ull || !sight.all(pa, pb, key, key + TILE - 1)) {
 #pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int j = 32 * n + result_row(r, lane);
-                    if (!(sight.one(pos, key + j) && (see >> j & 1))) s[n][r] = -__builtin_inff();
-                }
+            for (int n = 0; n < 2; n++) {
+                const uint32_t bits = visible16(sight, pos, key + 32 * n, (uint32_t)(see >> (32 * n)), lane);
+                hide(s[n], bits);
+            }
         }
         float top = s[0][0];
 #pragma unroll
@@ -312,7 +336,41 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
     if (lane < 32) a.lse[((int64_t)b * a.heads + head) * a.rows + t] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * LN2;
 }
 
-// Joins the parts of the keys: a workgroup a row, its waves every fourth part, a lane 2 elements.
+// Joins the parts of the keys, where they are few: a wave a row, a lane 2 elements.
+template <int DT>
+__global__ __launch_bounds__(256) void attn_join_few_kernel(AttnArgs a)
+{
+    const int total = a.rows * a.group, lane = threadIdx.x & 63, row = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (row >= total) return;
+    const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
+    const int64_t rows = (int64_t)gridDim.x * total, at_row = (int64_t)blockIdx.x * total + row;
+    const float *ml = a.partial + a.splits * rows * a.dim;
+    const int e = 2 * lane;
+    f32x2 p[FEW], v[FEW];
+#pragma unroll
+    for (int i = 0; i < FEW; i++) {
+        p[i] = i < a.splits ? *(const f32x2 *)(ml + (i * rows + at_row) * 2) : f32x2{-__builtin_inff(), 0.0f};
+        v[i] = i < a.splits && e < a.dim ? *(const f32x2 *)(a.partial + (i * rows + at_row) * a.dim + e) : f32x2{0.0f, 0.0f};
+    }
+    float m = p[0][0];
+#pragma unroll
+    for (int i = 1; i < FEW; i++) m = fmaxf(m, p[i][0]);
+    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < FEW; i++) {
+        const float w = exp2_hw(p[i][0] - ref);
+        l += w * p[i][1];
+        o0 += w * v[i][0];
+        o1 += w * v[i][1];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int t = row / a.group, head = hk * a.group + row % a.group;
+    if (e < a.dim) *(uint32_t *)((uint16_t *)at(a.o, b, head) + t * a.o.t + e) = pack2<DT>(o0 * inv, o1 * inv);
+    if (lane == 0) a.lse[((int64_t)b * a.heads + head) * a.rows + t] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * LN2;
+}
+
+// Joins many parts: a workgroup a row, its waves every fourth part, a lane 2 elements.
 template <int DT>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a)
 {
@@ -382,8 +440,13 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs a)
 }
 
 // A weight of all but 2^-16 leaves its row's other keys less than the rounding of `out` puts into
-// delta: the softmax is constant there and dS is 0 (exactly so where a row sees one key).
-__device__ __forceinline__ float score_gradient(float p, float dp, float delta) { return p > 1.0f - 0x1p-16f ? 0.0f : p * (dp - delta); }
+// delta: the softmax is constant there and dS is 0 (exactly so where a row sees one key).  A row
+// that sees that few keys meets them in tiles that are not all visible, the only ones to ask.
+__device__ __forceinline__ void settle(f32x16 &ds, const f32x16 &p, uint32_t visible)
+{
+#pragma unroll
+    for (int r = 0; r < 16; r++) ds[r] = (visible >> r & 1) && !(p[r] > 1.0f - 0x1p-16f) ? ds[r] : 0.0f;
+}
 
 // dq of WAVES x 32 rows: the forward pass's walk over the keys.
 template <int DT, int HD, int WAVES>
@@ -391,7 +454,7 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
 {
     constexpr int C = HD / 16, ND = HD / 32;
     __shared__ __attribute__((aligned(16))) char lds[2][TILE * Tile<HD>::ROW];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
     const int total = a.rows * a.group, r0 = (gridDim.y - 1 - blockIdx.y) * WAVES * 32, row = r0 + wave * 32 + (lane & 31);
     const Sight sight = {a.window, a.sinks};
@@ -428,37 +491,35 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
     next.load(a, b, hk, tiles.key(0));
     for (int it = 0; it < tiles.count; it++) {
         const int key = tiles.key(it);
-        const uint64_t see = next.see;
         __syncthreads();
-        next.store(lds[0], lds[1]);
+        const uint64_t see = next.store(a, lds[0], lds[1]);
         __syncthreads();
         if (it + 1 < tiles.count) next.load(a, b, hk, tiles.key(it + 1));
         if (see == 0 || sight.none(pa, pb, key, key + TILE - 1)) continue;
         const bool whole = see == ~0ull && sight.all(pa, pb, key, key + TILE - 1);
-#pragma unroll
         for (int n = 0; n < 2; n++) {
+            uint32_t bits = 0;                           // which of the lane's 16 results are visible
+            if (!whole) bits = visible16(sight, pos, key + 32 * n, (uint32_t)(see >> (32 * n)), lane);
+            __builtin_amdgcn_sched_barrier(0);
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                s = mma<DT>(Tile<HD>::rows(lds[0], 32 * n, c, lane), q[c], s);
-                dp = mma<DT>(Tile<HD>::rows(lds[1], 32 * n, c, lane), g[c], dp);
+                s = mma<DT>(Tile<HD>::rows(lds[0] + n * (32 * Tile<HD>::ROW), 0, c, lane), q[c], s);
+                dp = mma<DT>(Tile<HD>::rows(lds[1] + n * (32 * Tile<HD>::ROW), 0, c, lane), g[c], dp);
             }
-            if (whole) {
+            if (!whole) hide(s, bits);
 #pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = exp2_hw(__builtin_fmaf(s[r], c2, -lse)) * (dp[r] - delta);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int j = 32 * n + result_row(r, lane);
-                    const float p = exp2_hw(__builtin_fmaf(s[r], c2, -lse));
-                    s[r] = sight.one(pos, key + j) && (see >> j & 1) ? score_gradient(p, dp[r], delta) : 0.0f;
-                }
+            for (int r = 0; r < 16; r++) {
+                s[r] = exp2_hw(__builtin_fmaf(s[r], c2, -lse));
+                dp[r] = s[r] * (dp[r] - delta);
             }
+            if (!whole) settle(dp, s, bits);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                const u32x4 p = operand<DT>(s, 8 * k);
+                const u32x4 p = operand<DT>(dp, 8 * k);
 #pragma unroll
-                for (int d = 0; d < ND; d++) dq[d] = mma<DT>(Tile<HD>::columns(lds[0], 32 * n + 16 * k, d, lane), p, dq[d]);
+                for (int d = 0; d < ND; d++) dq[d] = mma<DT>(Tile<HD>::columns(lds[0] + n * (32 * Tile<HD>::ROW), 16 * k, d, lane), p, dq[d]);
             }
         }
     }
@@ -479,35 +540,45 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
 // positions whose window holds a key of its block; those behind that, which see the sinks alone, go to
 // workgroups of their own (DkvSplit), whose sums are fp32 partial results.
 template <int DT, int HD, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dkv_kernel(AttnArgs a, DkvSplit cut)
+__global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, DkvSplit cut)
 {
     constexpr int C = HD / 16, ND = HD / 32;
+    // the keys' v in registers where there is room, otherwise in LDS
+    constexpr bool VREGS = HD == 64;
     using S = Stage<HD, WAVES * 64, 32>;
     __shared__ __attribute__((aligned(16))) char lds[2][32 * Tile<HD>::ROW];
+    __shared__ __attribute__((aligned(16))) char vtile[VREGS ? 16 : WAVES * 32 * Tile<HD>::ROW];
     __shared__ __attribute__((aligned(16))) float lse_s[32], delta_s[32];
     __shared__ __attribute__((aligned(16))) int pos_s[32];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
     // blockIdx.y: the blocks of keys, then the sinks' far positions
     const int far = (int)blockIdx.y < cut.blocks ? -1 : ((int)blockIdx.y - cut.blocks) % cut.far;
     const int block = far < 0 ? blockIdx.y : (blockIdx.y - cut.blocks) / cut.far;
     const int k0 = block * WAVES * 32, ka = k0 + wave * 32, key = ka + (lane & 31);
     const Sight sight = {a.window, a.sinks};
-    const int before = a.keys - a.rows, total = a.rows * a.group;
+    const int before = a.keys - a.rows;
     const bool real = key < a.keys;
     const bool seen = real && (!a.key_mask || a.key_mask[b * a.mask_stride + key] != 0);
     const bool all_seen = __ballot(seen) == ~0ull;
 
-    u32x4 kf[C], vf[C];
+    u32x4 kf[C], vf[VREGS ? C : 1];
 #pragma unroll
     for (int c = 0; c < C; c++) {
         const int d = 16 * c + 8 * (lane >> 5);
-        kf[c] = vf[c] = u32x4{0, 0, 0, 0};
+        u32x4 v = {0, 0, 0, 0};
+        kf[c] = v;
         if (d < a.dim && seen) {
             kf[c] = *(const u32x4 *)(at(a.k, b, hk) + (int64_t)key * a.k.t + d);
-            vf[c] = *(const u32x4 *)(at(a.v, b, hk) + (int64_t)key * a.v.t + d);
+            v = *(const u32x4 *)(at(a.v, b, hk) + (int64_t)key * a.v.t + d);
         }
+        if constexpr (VREGS) vf[c] = v;
+        else *(u32x4 *)(vtile + (wave * 32 + (lane & 31)) * Tile<HD>::ROW + d * 2) = v;      // read by this wave alone
     }
+    auto values = [&](int c) {
+        if constexpr (VREGS) return vf[c];
+        else return Tile<HD>::rows(vtile, wave * 32, c, lane);
+    };
     f32x16 dk[ND], dv[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) dk[d] = dv[d] = zero16();
@@ -539,17 +610,12 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dkv_kernel(
         }
         qs.load(qr, [&](int i) { return qo[i]; });
         gs.load(gr, [&](int i) { return go[i]; });
-        if (threadIdx.x < 32) {
-            const int r = min(row0 + (int)threadIdx.x, total - 1), t = r / a.group;
-            const int64_t stat = ((int64_t)b * a.heads + hk * a.group + r - t * a.group) * a.rows + t;
-            lse_r = a.lse[stat] * LOG2E;
+        if (threadIdx.x < 32) {                          // (looked at when the tile is stored)
+            const int r = min(over + (int)threadIdx.x, last - 1 - row0 + over), t = (int)(((float)r + 0.5f) * per_group);
+            const int64_t stat = ((int64_t)b * a.heads + hk * a.group + r - t * a.group) * a.rows + t0 + t;
+            lse_r = a.lse[stat];
             delta_r = a.delta[stat];
-            // no weight where a row sees nothing, nor behind the last row
-            if (lse_r == -__builtin_inff() || row0 + (int)threadIdx.x >= last) {
-                lse_r = __builtin_inff();
-                delta_r = 0.0f;
-            }
-            pos_r = before + t;
+            pos_r = before + t0 + t;
         }
     };
     if (first < last) fetch(first);
@@ -558,8 +624,10 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dkv_kernel(
         qs.store(lds[0]);
         gs.store(lds[1]);
         if (threadIdx.x < 32) {
-            lse_s[threadIdx.x] = lse_r;
-            delta_s[threadIdx.x] = delta_r;
+            // no weight where a row sees nothing, nor behind the last row
+            const bool none = lse_r == -__builtin_inff() || row0 + (int)threadIdx.x >= last;
+            lse_s[threadIdx.x] = none ? __builtin_inff() : lse_r * LOG2E;
+            delta_s[threadIdx.x] = none ? 0.0f : delta_r;
             pos_s[threadIdx.x] = pos_r;
         }
         __syncthreads();
@@ -567,32 +635,33 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dkv_kernel(
         const int pa = before + row0 / a.group, pb = before + min(row0 + 31, last - 1) / a.group;
         if (sight.none(pa, pb, ka, ka + 31)) continue;
         const bool whole = all_seen && sight.all(pa, pb, ka, ka + 31);
+        uint32_t bits = 0;                               // which of the lane's 16 results are visible
+        if (!whole) {
+            for (int r = 0; r < 16; r += 4) {
+                const u32x4 po = *(const u32x4 *)(pos_s + result_row(r, lane));
+#pragma unroll
+                for (int k = 0; k < 4; k++) bits |= (uint32_t)(seen & sight.one((int)po[k], key)) << (r + k);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int c = 0; c < C; c++) {
             s = mma<DT>(Tile<HD>::rows(lds[0], 0, c, lane), kf[c], s);
-            dp = mma<DT>(Tile<HD>::rows(lds[1], 0, c, lane), vf[c], dp);
+            dp = mma<DT>(Tile<HD>::rows(lds[1], 0, c, lane), values(c), dp);
         }
+        if (!whole) hide(s, bits);
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-            const int i = result_row(r, lane);
-            const f32x4 ls = *(const f32x4 *)(lse_s + i), de = *(const f32x4 *)(delta_s + i);
-            if (whole) {
+            const f32x4 ls = *(const f32x4 *)(lse_s + result_row(r, lane)), de = *(const f32x4 *)(delta_s + result_row(r, lane));
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    s[r + k] = exp2_hw(__builtin_fmaf(s[r + k], c2, -ls[k]));
-                    dp[r + k] = s[r + k] * (dp[r + k] - de[k]);
-                }
-            } else {
-                const u32x4 po = *(const u32x4 *)(pos_s + i);
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float p = exp2_hw(__builtin_fmaf(s[r + k], c2, -ls[k]));
-                    s[r + k] = seen && sight.one((int)po[k], key) ? p : 0.0f;
-                    dp[r + k] = score_gradient(s[r + k], dp[r + k], de[k]);
-                }
+            for (int k = 0; k < 4; k++) {
+                s[r + k] = exp2_hw(__builtin_fmaf(s[r + k], c2, -ls[k]));
+                dp[r + k] = s[r + k] * (dp[r + k] - de[k]);
             }
         }
+        if (!whole) settle(dp, s, bits);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const u32x4 p = operand<DT>(s, 8 * k), ds = operand<DT>(dp, 8 * k);
@@ -656,7 +725,8 @@ void run_forward(const AttnArgs &a, hipStream_t stream)
         attn_fwd_kernel<DT, HD, 1><<<dim3(heads, 1, a.splits), 64, 0, stream>>>(a);
     else
         attn_fwd_kernel<DT, HD, 4><<<dim3(heads, (total + 127) / 128, a.splits), 256, 0, stream>>>(a);
-    if (a.splits > 1) attn_join_kernel<DT><<<dim3(heads, total), 256, 0, stream>>>(a);
+    if (a.splits > FEW) attn_join_kernel<DT><<<dim3(heads, total), 256, 0, stream>>>(a);
+    else if (a.splits > 1) attn_join_few_kernel<DT><<<dim3(heads, (total + 3) / 4), 256, 0, stream>>>(a);
 }
 
 template <int DT, int HD>
