@@ -16,9 +16,10 @@
 // rows of one column.  Softmax statistics then belong to lanes (a column is a row of the attention):
 // maximum and sum need one exchange between the wave's halves.
 //
-// LDS tiles are row major with 32 bytes between rows: eight lanes of a row read (8 rows, one 16-byte
-// piece each) and sixteen of a transposing read (4 rows x 32 bytes) then fall on different banks, and
-// every address is a lane's base plus a constant.
+// LDS tiles are row major, 16-byte pieces XOR-ed with their row: sixteen lanes of a row read (16 rows,
+// one piece each) and sixteen of a transposing read (4 rows x 2 pieces) then fall on different ones
+// of the 64 banks (with 32 bytes between rows instead the row reads took twice the cycles).  Tiles
+// come in pairs, one read while the other is filled: one barrier a tile.
 #pragma once
 #include "lm_attn.h"
 #include "lm_common.h"
@@ -55,24 +56,36 @@ __device__ __forceinline__ f32x16 zero16()
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
-// A tile of rows of HD 16-bit elements in LDS, 32 bytes between rows.
+// A tile of rows of HD 16-bit elements in LDS, aligned to its rows.  `t` is the tile's offset in LDS.
+typedef __attribute__((address_space(3))) char lds_char;
 template <int HD>
 struct Tile {
-    static constexpr int ROW = HD * 2 + 32;
+    static constexpr int ROW = HD * 2;
 
-    // A operand, its k along the elements: row `row` + lane & 31, elements 16 c + 8 half ...
-    static __device__ __forceinline__ u32x4 rows(const char *t, int row, int c, int lane)
+    static __device__ __forceinline__ int turn(int row)
     {
-        return *(const u32x4 *)(t + ((lane & 31) * ROW + (lane >> 5) * 16) + (row * ROW + c * 32));
+        return (HD == 128 ? ((row & 7) << 1) | ((row >> 3) & 1) : (row & 6) | ((row >> 3) & 1)) << 4;
+    }
+    static __device__ __forceinline__ int at(int row, int piece) { return row * ROW + ((piece << 4) ^ turn(row)); }
+
+    // A lane's place in the tile for each kind of read; what differs between reads are constants.
+    static __device__ __forceinline__ int row_place(int lane) { return at(lane & 31, lane >> 5); }
+    static __device__ __forceinline__ int column_place(int lane)
+    {
+        return at(4 * (lane >> 5) + ((lane >> 2) & 3), ((lane >> 3) & 2) + ((lane >> 1) & 1)) + (lane & 1) * 8;
+    }
+    // A operand, its k along the elements: row `row` + lane & 31, elements 16 c + 8 half ...
+    static __device__ __forceinline__ u32x4 rows(const lds_char *t, int place, int row, int c)
+    {
+        return *(const __attribute__((address_space(3))) u32x4 *)(t + (place ^ (c << 5)) + row * ROW);
     }
     // A operand, its k along the rows: element 32 d + lane & 31 of the 16 rows from `row`, in the
     // order of a result's registers
-    static __device__ __forceinline__ u32x4 columns(const char *t, int row, int d, int lane)
+    static __device__ __forceinline__ u32x4 columns(const lds_char *t, int place, int row, int d)
     {
         typedef __attribute__((address_space(3))) s16x4 *lds4;
-        const char *p = t + ((4 * (lane >> 5) + ((lane >> 2) & 3)) * ROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8) + (row * ROW + d * 64);
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 8 * ROW));
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(t + (place ^ (d << 6)) + row * ROW));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(t + (place ^ (d << 6 | 16)) + (row + 8) * ROW));
         const u32x2 u = __builtin_bit_cast(u32x2, x), w = __builtin_bit_cast(u32x2, y);
         return u32x4{u[0], u[1], w[0], w[1]};
     }
@@ -84,6 +97,15 @@ __device__ __forceinline__ u32x4 operand(const f32x16 &s, int r0)
 {
     return u32x4{pack2<DT>(s[r0], s[r0 + 1]), pack2<DT>(s[r0 + 2], s[r0 + 3]), pack2<DT>(s[r0 + 4], s[r0 + 5]),
                  pack2<DT>(s[r0 + 6], s[r0 + 7])};
+}
+
+// Waits for loaded registers here.  Loads that are first used inside a loop are otherwise waited for
+// there, on every turn, and with them the loop's own loads for its next turn.
+template <int N>
+__device__ __forceinline__ void landed(u32x4 (&v)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+v"(v[i]));
 }
 
 // The row of a result's register r within its 32.
@@ -163,10 +185,14 @@ struct Stage {
         for (int i = 0; i < N; i++)
             v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, offset(i), 0, 0));
     }
-    __device__ __forceinline__ void store(char *tile) const
+    __device__ __forceinline__ void store(lds_char *tile) const
     {
 #pragma unroll
-        for (int i = 0; i < N; i++) *(u32x4 *)(tile + (row() + i * STEP) * Tile<HD>::ROW + piece() * 16) = v[i];
+        for (int i = 0; i < N; i++) {
+            // (STEP rows on, the row's turn is the same where STEP is a multiple of 16)
+            const int at = STEP % 16 ? Tile<HD>::at(row() + i * STEP, piece()) : Tile<HD>::at(row(), piece()) + i * STEP * Tile<HD>::ROW;
+            *(__attribute__((address_space(3))) u32x4 *)(tile + at) = v[i];
+        }
     }
 };
 
@@ -198,7 +224,7 @@ struct KeyStage {
         }
     }
     // Returns which keys are shown; the hidden ones' rows are zero.
-    __device__ __forceinline__ uint64_t store(const AttnArgs &a, char *ktile, char *vtile)
+    __device__ __forceinline__ uint64_t store(const AttnArgs &a, lds_char *ktile, lds_char *vtile)
     {
         const uint64_t see = a.key_mask ? __ballot(mask != 0) : ~0ull;
         if (see != ~0ull) {
@@ -220,7 +246,9 @@ template <int DT, int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void attn_fwd_kernel(AttnArgs a)
 {
     constexpr int C = HD / 16, ND = HD / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2][TILE * Tile<HD>::ROW];
+    constexpr int BYTES = TILE * Tile<HD>::ROW;
+    __shared__ __attribute__((aligned(256))) char lds_[4 * BYTES];          // k, v; k, v of the next tile
+    lds_char *const lds = (lds_char *)lds_;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
     const int total = a.rows * a.group, r0 = (gridDim.y - 1 - blockIdx.y) * WAVES * 32, row = r0 + wave * 32 + (lane & 31);
@@ -244,26 +272,33 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
     const KeyTiles tiles(a, before + r0 / a.group, before + min(r0 + WAVES * 32 - 1, total - 1) / a.group);
     const int per = (tiles.count + a.splits - 1) / a.splits, it0 = blockIdx.z * per, it1 = min(tiles.count, it0 + per);
 
+    landed(q);
     f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = zero16();
     float m = -__builtin_inff(), l = 0.0f;         // in units of log2; l of this lane's keys alone
     const float c2 = a.scale * LOG2E;
     KeyStage<HD, WAVES * 64> next;
-    if (it0 < it1) next.load(a, b, hk, tiles.key(it0));
+    int rp = Tile<HD>::row_place(lane), cp = Tile<HD>::column_place(lane);
+    uint64_t see = 0;
+    int turn = 0;                                  // the tile being read
+    if (it0 < it1) {
+        next.load(a, b, hk, tiles.key(it0));
+        see = next.store(a, lds, lds + BYTES);
+        if (it0 + 1 < it1) next.load(a, b, hk, tiles.key(it0 + 1));
+    }
+    __syncthreads();
     for (int it = it0; it < it1; it++) {
         const int key = tiles.key(it);
-        __syncthreads();
-        const uint64_t see = next.store(a, lds[0], lds[1]);
-        __syncthreads();
-        if (it + 1 < it1) next.load(a, b, hk, tiles.key(it + 1));
-        if (see == 0 || sight.none(pa, pb, key, key + TILE - 1)) continue;
+        const lds_char *kt = lds + turn, *vt = kt + BYTES;
+        asm volatile("" : "+v"(rp), "+v"(cp));     // the reads' addresses are formed where they are used, not kept
+        if (see != 0 && !sight.none(pa, pb, key, key + TILE - 1)) {
 
         f32x16 s[2] = {zero16(), zero16()};
 #pragma unroll
         for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int n = 0; n < 2; n++) s[n] = mma<DT>(Tile<HD>::rows(lds[0], 32 * n, c, lane), q[c], s[n]);
+            for (int n = 0; n < 2; n++) s[n] = mma<DT>(Tile<HD>::rows(kt, rp, 32 * n, c), q[c], s[n]);
         if (see != ~0ull || !sight.all(pa, pb, key, key + TILE - 1)) {
 #pragma unroll
             for (int n = 0; n < 2; n++) {
@@ -301,8 +336,15 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
             for (int k = 0; k < 2; k++) {
                 const u32x4 p = operand<DT>(s[n], 8 * k);
 #pragma unroll
-                for (int d = 0; d < ND; d++) o[d] = mma<DT>(Tile<HD>::columns(lds[1], 32 * n + 16 * k, d, lane), p, o[d]);
+                for (int d = 0; d < ND; d++) o[d] = mma<DT>(Tile<HD>::columns(vt, cp, 32 * n + 16 * k, d), p, o[d]);
             }
+        }
+        turn ^= 2 * BYTES;
+        if (it + 1 < it1) {
+            see = next.store(a, lds + turn, lds + turn + BYTES);
+            if (it + 2 < it1) next.load(a, b, hk, tiles.key(it + 2));
+        }
+        __syncthreads();
     }
     l += other_half(l);
     if (!real) return;
@@ -453,7 +495,9 @@ template <int DT, int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a)
 {
     constexpr int C = HD / 16, ND = HD / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2][TILE * Tile<HD>::ROW];
+    constexpr int BYTES = TILE * Tile<HD>::ROW;
+    __shared__ __attribute__((aligned(256))) char lds_[4 * BYTES];          // k, v; k, v of the next tile
+    lds_char *const lds = (lds_char *)lds_;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
     const int total = a.rows * a.group, r0 = (gridDim.y - 1 - blockIdx.y) * WAVES * 32, row = r0 + wave * 32 + (lane & 31);
@@ -478,24 +522,31 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
     const int64_t stat = ((int64_t)b * a.heads + head) * a.rows + t;
     float lse = a.lse[stat] * LOG2E;
     if (lse == -__builtin_inff()) lse = __builtin_inff();          // an empty row: every weight 0
-    const float delta = a.delta[stat];
+    float delta = a.delta[stat];
     const int wa = min(r0 + wave * 32, total - 1), wb = min(r0 + wave * 32 + 31, total - 1);
     const int pa = __builtin_amdgcn_readfirstlane(before + wa / a.group), pb = __builtin_amdgcn_readfirstlane(before + wb / a.group);
     const KeyTiles tiles(a, before + r0 / a.group, before + min(r0 + WAVES * 32 - 1, total - 1) / a.group);
 
+    landed(q);
+    landed(g);
+    asm volatile("" : "+v"(lse), "+v"(delta));
     f32x16 dq[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) dq[d] = zero16();
     const float c2 = a.scale * LOG2E;
     KeyStage<HD, WAVES * 64> next;
+    int rp = Tile<HD>::row_place(lane), cp = Tile<HD>::column_place(lane);
+    uint64_t see = 0;
+    int turn = 0;                                  // the tile being read
     next.load(a, b, hk, tiles.key(0));
+    see = next.store(a, lds, lds + BYTES);
+    if (tiles.count > 1) next.load(a, b, hk, tiles.key(1));
+    __syncthreads();
     for (int it = 0; it < tiles.count; it++) {
         const int key = tiles.key(it);
-        __syncthreads();
-        const uint64_t see = next.store(a, lds[0], lds[1]);
-        __syncthreads();
-        if (it + 1 < tiles.count) next.load(a, b, hk, tiles.key(it + 1));
-        if (see == 0 || sight.none(pa, pb, key, key + TILE - 1)) continue;
+        const lds_char *kt = lds + turn, *vt = kt + BYTES;
+        asm volatile("" : "+v"(rp), "+v"(cp));     // the reads' addresses are formed where they are used, not kept
+        if (see != 0 && !sight.none(pa, pb, key, key + TILE - 1)) {
         const bool whole = see == ~0ull && sight.all(pa, pb, key, key + TILE - 1);
         for (int n = 0; n < 2; n++) {
             uint32_t bits = 0;                           // which of the lane's 16 results are visible
@@ -504,8 +555,8 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                s = mma<DT>(Tile<HD>::rows(lds[0] + n * (32 * Tile<HD>::ROW), 0, c, lane), q[c], s);
-                dp = mma<DT>(Tile<HD>::rows(lds[1] + n * (32 * Tile<HD>::ROW), 0, c, lane), g[c], dp);
+                s = mma<DT>(Tile<HD>::rows(kt + n * (32 * Tile<HD>::ROW), rp, 0, c), q[c], s);
+                dp = mma<DT>(Tile<HD>::rows(vt + n * (32 * Tile<HD>::ROW), rp, 0, c), g[c], dp);
             }
             if (!whole) hide(s, bits);
 #pragma unroll
@@ -519,9 +570,16 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
             for (int k = 0; k < 2; k++) {
                 const u32x4 p = operand<DT>(dp, 8 * k);
 #pragma unroll
-                for (int d = 0; d < ND; d++) dq[d] = mma<DT>(Tile<HD>::columns(lds[0] + n * (32 * Tile<HD>::ROW), 16 * k, d, lane), p, dq[d]);
+                for (int d = 0; d < ND; d++) dq[d] = mma<DT>(Tile<HD>::columns(kt + n * (32 * Tile<HD>::ROW), cp, 16 * k, d), p, dq[d]);
             }
         }
+        }
+        turn ^= 2 * BYTES;
+        if (it + 1 < tiles.count) {
+            see = next.store(a, lds + turn, lds + turn + BYTES);
+            if (it + 2 < tiles.count) next.load(a, b, hk, tiles.key(it + 2));
+        }
+        __syncthreads();
     }
     if (!real) return;
     uint16_t *po = (uint16_t *)at(a.dq, b, head) + t * a.dq.t;
@@ -546,10 +604,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
     // the keys' v in registers where there is room, otherwise in LDS
     constexpr bool VREGS = HD == 64;
     using S = Stage<HD, WAVES * 64, 32>;
-    __shared__ __attribute__((aligned(16))) char lds[2][32 * Tile<HD>::ROW];
-    __shared__ __attribute__((aligned(16))) char vtile[VREGS ? 16 : WAVES * 32 * Tile<HD>::ROW];
-    __shared__ __attribute__((aligned(16))) float lse_s[32], delta_s[32];
-    __shared__ __attribute__((aligned(16))) int pos_s[32];
+    constexpr int BYTES = 32 * Tile<HD>::ROW;
+    __shared__ __attribute__((aligned(256))) char lds_[4 * BYTES + (VREGS ? 0 : WAVES * BYTES)];   // q, dout; q, dout of the next tile; v
+    __shared__ __attribute__((aligned(16))) float lse_s[2][32], delta_s[2][32];
+    __shared__ __attribute__((aligned(16))) int pos_s[2][32];
+    lds_char *const lds = (lds_char *)lds_;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
     // blockIdx.y: the blocks of keys, then the sinks' far positions
@@ -562,6 +621,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
     const bool seen = real && (!a.key_mask || a.key_mask[b * a.mask_stride + key] != 0);
     const bool all_seen = __ballot(seen) == ~0ull;
 
+    lds_char *const vtile = lds + (4 + wave) * BYTES;
+    int rp = Tile<HD>::row_place(lane), cp = Tile<HD>::column_place(lane);
     u32x4 kf[C], vf[VREGS ? C : 1];
 #pragma unroll
     for (int c = 0; c < C; c++) {
@@ -573,12 +634,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
             v = *(const u32x4 *)(at(a.v, b, hk) + (int64_t)key * a.v.t + d);
         }
         if constexpr (VREGS) vf[c] = v;
-        else *(u32x4 *)(vtile + (wave * 32 + (lane & 31)) * Tile<HD>::ROW + d * 2) = v;      // read by this wave alone
+        else *(__attribute__((address_space(3))) u32x4 *)(vtile + Tile<HD>::at(lane & 31, 2 * c + (lane >> 5))) = v;      // read by this wave alone
     }
     auto values = [&](int c) {
         if constexpr (VREGS) return vf[c];
-        else return Tile<HD>::rows(vtile, wave * 32, c, lane);
+        else return Tile<HD>::rows(vtile, rp, 0, c);
     };
+    landed(kf);
+    if constexpr (VREGS) landed(vf);
     f32x16 dk[ND], dv[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) dk[d] = dv[d] = zero16();
@@ -596,64 +659,85 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
     float lse_r = 0.0f, delta_r = 0.0f;
     int pos_r = 0;
     const float per_group = 1.0f / (float)a.group;
-    auto fetch = [&](int row0) {
-        // row0 + r is position t0 + (over + r) / group: small numbers, divided in fp32
-        const int t0 = row0 / a.group, over = row0 - t0 * a.group;
-        const auto qr = buffer_from(at(a.q, b, hk * a.group) + t0 * a.q.t), gr = buffer_from(at(a.dout, b, hk * a.group) + t0 * a.dout.t);
+    const uint16_t *const qp = at(a.q, b, hk * a.group), *const gp = at(a.dout, b, hk * a.group);
+    // the next tile to bring: its first row is head `over` of position t0 (a tile on is `whole_t` positions
+    // and `rest` heads on)
+    int t0 = p0 - before, over = 0, row_in = first;
+    const int whole_t = 32 / a.group, rest = 32 - whole_t * a.group;
+    auto fetch = [&]() {
+        const auto qr = buffer_from(qp + t0 * a.q.t), gr = buffer_from(gp + t0 * a.dout.t);
         uint32_t qo[S::N], go[S::N];
 #pragma unroll
         for (int i = 0; i < S::N; i++) {
-            const int r = S::row() + i * S::STEP, t = (int)(((float)(over + r) + 0.5f) * per_group), g = over + r - t * a.group;
-            const bool there = row0 + r < last && S::piece() * 8 < a.dim;
+            // small numbers, divided in fp32
+            const int r = over + S::row() + i * S::STEP, t = (int)(((float)r + 0.5f) * per_group), g = r - t * a.group;
+            const bool there = row_in + S::row() + i * S::STEP < last && S::piece() * 8 < a.dim;
             qo[i] = there ? (t * (uint32_t)a.q.t + g * (uint32_t)a.q.h + S::piece() * 8) * 2 : NOWHERE;
             go[i] = there ? (t * (uint32_t)a.dout.t + g * (uint32_t)a.dout.h + S::piece() * 8) * 2 : NOWHERE;
         }
         qs.load(qr, [&](int i) { return qo[i]; });
         gs.load(gr, [&](int i) { return go[i]; });
         if (threadIdx.x < 32) {                          // (looked at when the tile is stored)
-            const int r = min(over + (int)threadIdx.x, last - 1 - row0 + over), t = (int)(((float)r + 0.5f) * per_group);
-            const int64_t stat = ((int64_t)b * a.heads + hk * a.group + r - t * a.group) * a.rows + t0 + t;
+            const int r = over + min((int)threadIdx.x, last - 1 - row_in), t = (int)(((float)r + 0.5f) * per_group), g = r - t * a.group;
+            const int64_t stat = ((int64_t)b * a.heads + hk * a.group + g) * a.rows + t0 + t;
             lse_r = a.lse[stat];
             delta_r = a.delta[stat];
             pos_r = before + t0 + t;
+            // behind the last row there is no weight
+            if (row_in + (int)threadIdx.x >= last) pos_r = -1;
+        }
+        row_in += 32;
+        t0 += whole_t;
+        over += rest;
+        if (over >= a.group) {
+            over -= a.group;
+            t0++;
         }
     };
-    if (first < last) fetch(first);
-    for (int row0 = first; row0 < last; row0 += 32) {
-        __syncthreads();
-        qs.store(lds[0]);
-        gs.store(lds[1]);
+    auto store = [&](int side) {
+        qs.store(lds + side * 2 * BYTES);
+        gs.store(lds + side * 2 * BYTES + BYTES);
         if (threadIdx.x < 32) {
-            // no weight where a row sees nothing, nor behind the last row
-            const bool none = lse_r == -__builtin_inff() || row0 + (int)threadIdx.x >= last;
-            lse_s[threadIdx.x] = none ? __builtin_inff() : lse_r * LOG2E;
-            delta_s[threadIdx.x] = none ? 0.0f : delta_r;
-            pos_s[threadIdx.x] = pos_r;
+            const bool none = pos_r < 0 || lse_r == -__builtin_inff();   // nor where a row sees nothing
+            lse_s[side][threadIdx.x] = none ? __builtin_inff() : lse_r * LOG2E;
+            delta_s[side][threadIdx.x] = none ? 0.0f : delta_r;
+            pos_s[side][threadIdx.x] = pos_r;
         }
-        __syncthreads();
-        if (row0 + 32 < last) fetch(row0 + 32);
-        const int pa = before + row0 / a.group, pb = before + min(row0 + 31, last - 1) / a.group;
-        if (sight.none(pa, pb, ka, ka + 31)) continue;
+    };
+    int side = 0;
+    // the positions of the tile being read: pa, and no more than pb
+    int pa = p0, pb = p0;
+    if (first < last) {
+        fetch();
+        pb = before + t0;
+        store(0);
+        if (row_in < last) fetch();
+    }
+    __syncthreads();
+    for (int row0 = first; row0 < last; row0 += 32) {
+        const lds_char *qt = lds + side * 2 * BYTES, *gt = qt + BYTES;
+        asm volatile("" : "+v"(rp), "+v"(cp));     // the reads' addresses are formed where they are used, not kept
+        if (!sight.none(pa, pb, ka, ka + 31)) {
         const bool whole = all_seen && sight.all(pa, pb, ka, ka + 31);
         uint32_t bits = 0;                               // which of the lane's 16 results are visible
         if (!whole) {
             for (int r = 0; r < 16; r += 4) {
-                const u32x4 po = *(const u32x4 *)(pos_s + result_row(r, lane));
+                const u32x4 po = *(const u32x4 *)(pos_s[side] + result_row(r, lane));
 #pragma unroll
-                for (int k = 0; k < 4; k++) bits |= (uint32_t)(seen & sight.one((int)po[k], key)) << (r + k);
+                for (int k = 0; k < 4; k++) bits |= (uint32_t)(seen && sight.one((int)po[k], key)) << (r + k);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            s = mma<DT>(Tile<HD>::rows(lds[0], 0, c, lane), kf[c], s);
-            dp = mma<DT>(Tile<HD>::rows(lds[1], 0, c, lane), values(c), dp);
+            s = mma<DT>(Tile<HD>::rows(qt, rp, 0, c), kf[c], s);
+            dp = mma<DT>(Tile<HD>::rows(gt, rp, 0, c), values(c), dp);
         }
         if (!whole) hide(s, bits);
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-            const f32x4 ls = *(const f32x4 *)(lse_s + result_row(r, lane)), de = *(const f32x4 *)(delta_s + result_row(r, lane));
+            const f32x4 ls = *(const f32x4 *)(lse_s[side] + result_row(r, lane)), de = *(const f32x4 *)(delta_s[side] + result_row(r, lane));
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 s[r + k] = exp2_hw(__builtin_fmaf(s[r + k], c2, -ls[k]));
@@ -667,10 +751,19 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
             const u32x4 p = operand<DT>(s, 8 * k), ds = operand<DT>(dp, 8 * k);
 #pragma unroll
             for (int d = 0; d < ND; d++) {
-                dv[d] = mma<DT>(Tile<HD>::columns(lds[1], 16 * k, d, lane), p, dv[d]);
-                dk[d] = mma<DT>(Tile<HD>::columns(lds[0], 16 * k, d, lane), ds, dk[d]);
+                dv[d] = mma<DT>(Tile<HD>::columns(gt, cp, 16 * k, d), p, dv[d]);
+                dk[d] = mma<DT>(Tile<HD>::columns(qt, cp, 16 * k, d), ds, dk[d]);
             }
         }
+        }
+        side ^= 1;
+        pa = pb;
+        if (row0 + 32 < last) {
+            pb = before + t0;
+            store(side);
+            if (row_in < last) fetch();
+        }
+        __syncthreads();
     }
     if (!real) return;
     if (cut.far && key < a.sinks) {
