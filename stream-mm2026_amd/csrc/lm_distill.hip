@@ -18,7 +18,11 @@
 namespace lm {
 namespace {
 
-constexpr float LOG2E = 1.44269504088896340736f;
+// Rows that together outgrow the last-level cache pass it by (non-temporal accesses).
+constexpr int NT = 2;
+constexpr int64_t BIG = 128 << 20;
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 __device__ __forceinline__ int64_t index_at(const void *p, int bytes, int64_t i)
 {
@@ -27,10 +31,14 @@ __device__ __forceinline__ int64_t index_at(const void *p, int bytes, int64_t i)
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// A row's teacher entries: what each thread would otherwise keep in registers over the passes.
 struct RowLds {
-    float buf[4][16];
-    int ids[DISTILL_MAX_K];
-    float p[DISTILL_MAX_K];
+    int ids[DISTILL_MAX_K];          // -1: absent
+    float t[DISTILL_MAX_K];          // teacher logit / T, then its log weight
+    float p[DISTILL_MAX_K];          // weight
+    float z[DISTILL_MAX_K];          // the student's logit
+    float w[DISTILL_MAX_K];          // the weights of all entries with this id, at its first entry; elsewhere -1
+    float top[16], sum[3][16];
 };
 
 // How a row lies in memory: `head` single elements, `pieces` whole 16-byte pieces, `tail` single ones.
@@ -52,34 +60,68 @@ __device__ __forceinline__ RowShape row_shape(const void *base, int64_t first, i
     return s;
 }
 
+// exp(z - max) of N values from exp((z - max) / T): the T-th power, where T is 1, 2 or 4 (a
+// multiplication or two in place of an exponential, which costs four; `pow` 0: formed by itself).
+template <int N>
+__device__ __forceinline__ void at_one(int pow, const float *e, const float *z, float m1, float *o)
+{
+    if (pow == 0) {
+#pragma unroll
+        for (int j = 0; j < N; j++) o[j] = exp2_hw(__builtin_fmaf(z[j], LOG2E, -m1));
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) o[j] = pow == 1 ? e[j] : e[j] * e[j];
+        if (pow == 4)
+#pragma unroll
+            for (int j = 0; j < N; j++) o[j] *= o[j];
+    }
+}
+
+// The memory from p on, `bytes` of it, for buffer accesses (beyond it: zeros read, nothing written).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_from(const void *p, uint32_t bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, bytes, 0x00027000);
+}
+
 // MODE 0: loss (and stats); 1: loss and gradient; 2: gradient from stats.  NC: pieces a thread
 // keeps in registers (0: none, the row is read again).
-template <int DT, int MODE, int THREADS, int NC>
-__global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs a)
+template <int DT, int MODE, int THREADS, int NC, int WAVES_PER_SIMD, int AUX>
+__global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(DistillArgs a)
 {
+    __shared__ RowLds s;
     using E = Elem<DT>;
     constexpr int W = THREADS / 64, P = E::PER16;
-    __shared__ RowLds s;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63;
     const int64_t n = blockIdx.x;
     const int vocab = (int)a.vocab;
     const RowShape sh = row_shape<DT>(a.logits, n * a.stride, vocab);
     const u32x4 *body = (const u32x4 *)(sh.row + sh.head * E::SIZE);
-    const float invT = 1.0f / a.temperature;
-    const bool has_label = a.labels != nullptr;
+    const float invT = 1.0f / a.temperature, cT = invT * LOG2E;
+    const int pow = a.temperature == 1.0f ? 1 : a.temperature == 2.0f ? 2 : a.temperature == 4.0f ? 4 : 0;
 
-    // the teacher's entries: one a thread where there are as many threads
+    // the row, on its way while the teacher's entries are looked at
+    u32x4 reg[NC ? NC : 1];
+    if constexpr (NC > 0) {
+        const auto from = buffer_from(body, sh.pieces * 16);
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+            reg[c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, tid * 16, c * THREADS * 16, AUX));
+    }
+    // each single element of head and tail is one thread's (there are fewer than 2 P of them)
+    const int edge = tid < sh.head ? tid : tid < sh.head + sh.tail ? vocab - sh.tail + (tid - sh.head) : -1;
+    const float zedge = edge >= 0 ? E::load(sh.row, edge) : -__builtin_inff();
+
     int any = 0;
     for (int k = tid; k < a.k; k += THREADS) {
         const int64_t id = index_at(a.ids, a.id_bytes, n * a.k + k);
         const bool there = id >= 0 && id < vocab;
         s.ids[k] = there ? (int)id : -1;
-        s.p[k] = there ? load_any(a.teacher_dt, a.teacher, n * a.k + k) * invT : -__builtin_inff();
+        s.t[k] = there ? load_any(a.teacher_dt, a.teacher, n * a.k + k) * invT : -__builtin_inff();
         any |= there;
     }
-    const bool taught = __syncthreads_or(any) && a.alpha != 0.0f;
-    int64_t label = has_label ? index_at(a.labels, a.label_bytes, n) : -1;
+    const int64_t label = a.labels ? index_at(a.labels, a.label_bytes, n) : -1;
     const bool named = label >= 0 && label < vocab && a.alpha != 1.0f;
+    const bool taught = __syncthreads_or(any) && a.alpha != 0.0f;
     const float wd = taught ? a.alpha : 0.0f, wl = named ? 1.0f - a.alpha : 0.0f;
 
     // dlogits' pieces are those of the logits where both rows start alike in their 16 bytes
@@ -99,40 +141,54 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs a)
                 else
                     for (int j = 0; j < P; j++) E::store(drow, sh.head + i * P + j, 0.0f);
             }
-            for (int i = tid; i < sh.head + sh.tail; i += THREADS)
-                E::store(drow, i < sh.head ? i : vocab - sh.tail + (i - sh.head), 0.0f);
+            if (edge >= 0) E::store(drow, edge, 0.0f);
         }
         return;
     }
 
-    // the row
-    u32x4 reg[NC ? NC : 1];
-    if constexpr (NC > 0) {
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const int i = tid + c * THREADS;
-            if (i < sh.pieces) reg[c] = body[i];
-        }
-    }
-    // each single element of head and tail is one thread's (there are fewer than 2 P of them)
-    const int edge = tid < sh.head ? tid : tid < sh.head + sh.tail ? vocab - sh.tail + (tid - sh.head) : -1;
-    const float zedge = edge >= 0 ? E::load(sh.row, edge) : -__builtin_inff();
     // the logits at the teacher's entries and the label, read before a gradient may overwrite them
-    constexpr int KPT = (DISTILL_MAX_K + THREADS - 1) / THREADS;
-    float zk[KPT];
-#pragma unroll
-    for (int u = 0; u < KPT; u++) {
-        const int k = tid + u * THREADS;
-        zk[u] = k < a.k && s.ids[k] >= 0 ? E::load(sh.row, s.ids[k]) : 0.0f;
-    }
+    for (int k = tid; k < a.k; k += THREADS) s.z[k] = s.ids[k] >= 0 ? E::load(sh.row, s.ids[k]) : 0.0f;
     const float zl = named ? E::load(sh.row, label) : 0.0f;
 
-    auto each = [&](auto f) {            // f(value index of the piece, its values)
+    // the teacher's distribution: its normaliser in every wave, the weights in LDS
+    bool label_there = false;
+    if (taught) {
+        float m = -__builtin_inff();
+        for (int k = lane; k < a.k; k += 64) m = Max()(m, s.t[k]);
+        m = wave_reduce(m, Max());
+        const float ref = m == -__builtin_inff() ? 0.0f : m;
+        float z = 0.0f;
+        for (int k = lane; k < a.k; k += 64) z += expf(s.t[k] - ref);
+        z = wave_reduce(z, Add());
+        const float logz = z > 0.0f || z != z ? logf(z) : __builtin_inff();      // every entry at -inf: all weights 0
+        __syncthreads();
+        for (int k = tid; k < a.k; k += THREADS) {
+            s.t[k] = s.t[k] - ref - logz;
+            s.p[k] = expf(s.t[k]);
+        }
+        __syncthreads();
+        // an id that comes more than once is its first entry's to write, with all weights
+        if (MODE != 0)
+            for (int k = tid; k < a.k; k += THREADS) {
+                const int id = s.ids[k];
+                float w = id < 0 ? -1.0f : 0.0f;
+                if (id >= 0)
+                    for (int j = 0; j < a.k; j++)
+                        if (s.ids[j] == id) w = j < k ? -1.0f : w < 0.0f ? w : w + s.p[j];
+                s.w[k] = w;
+                label_there |= id == (int)label;
+            }
+    }
+
+    // a value stays packed between its uses: unpacked once and kept, the row would take twice the
+    // registers and the CU half the rows
+    auto each = [&](auto f) {            // f(index of the piece, its values)
         float v[P];
         if constexpr (NC > 0) {
 #pragma unroll
             for (int c = 0; c < NC; c++) {
                 const int i = tid + c * THREADS;
+                asm volatile("" : "+v"(reg[c]));
                 if (i < sh.pieces) {
                     E::unpack(reg[c], v);
                     f(i, v);
@@ -146,8 +202,9 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs a)
         }
     };
 
+    // exponents are z c - top c in one rounding; what rounding top c loses is the same for every value
+    // of the row and goes out with the sums
     float top, lse_t, lse_1;             // the row's maximum and the two log-sums below it
-    const float cT = invT * LOG2E;
     if constexpr (MODE == 2) {
         top = a.stats[n * 4];
         lse_t = a.stats[n * 4 + 1];
@@ -156,61 +213,59 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs a)
         float m = zedge;
         each([&](int, float *v) {
 #pragma unroll
-            for (int j = 0; j < P; j++) m = Max()(m, v[j]);
+            for (int j = 0; j < P; j += 2) m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(v[j], v[j + 1]), m);
         });
-        top = group_reduce<W>(m, Max(), s.buf[0]);
-        float st = 0.0f, s1 = 0.0f;
-        if (taught) {
-            st = edge >= 0 ? exp2_hw((zedge - top) * cT) : 0.0f;
-            each([&](int, float *v) {
-#pragma unroll
-                for (int j = 0; j < P; j++) st += exp2_hw((v[j] - top) * cT);
-            });
-        }
-        if (named) {
-            s1 = edge >= 0 ? exp2_hw((zedge - top) * LOG2E) : 0.0f;
-            each([&](int, float *v) {
-#pragma unroll
-                for (int j = 0; j < P; j++) s1 += exp2_hw((v[j] - top) * LOG2E);
-            });
-        }
-        lse_t = taught ? logf(group_reduce<W>(st, Add(), s.buf[1])) : 0.0f;
-        lse_1 = named ? logf(group_reduce<W>(s1, Add(), s.buf[2])) : 0.0f;
+        top = group_reduce<W>(m, Max(), s.top);
     }
-
-    // the teacher's distribution (every wave forms it: k values in LDS)
-    float logz = 0.0f, tmax = -__builtin_inff();
-    if (taught) {
-        float m = -__builtin_inff();
-        for (int k = tid & 63; k < a.k; k += 64)
-            if (s.ids[k] >= 0) m = Max()(m, s.p[k]);
-        tmax = wave_reduce(m, Max());
-        const float ref = tmax == -__builtin_inff() ? 0.0f : tmax;
-        float z = 0.0f;
-        for (int k = tid & 63; k < a.k; k += 64)
-            if (s.ids[k] >= 0) z += expf(s.p[k] - ref);
-        z = wave_reduce(z, Add());
-        tmax = ref;
-        logz = z > 0.0f || z != z ? logf(z) : __builtin_inff();      // every entry at -inf: all weights 0
-    }
-    if (MODE != 2 && (a.loss || a.stats)) {
-        float kd = 0.0f;
-        if (taught) {
+    const float mT = top * cT, m1 = top * LOG2E;
+    if constexpr (MODE != 2) {
+        float st = 0.0f, s1 = 0.0f, kd = 0.0f;
+        if (edge >= 0) {
+            st = exp2_hw(__builtin_fmaf(zedge, cT, -mT));
+            if (named) at_one<1>(pow, &st, &zedge, m1, &s1);
+        }
+        each([&](int, float *v) {
+            float e[P], o[P];
 #pragma unroll
-            for (int u = 0; u < KPT; u++) {
-                const int k = tid + u * THREADS;
-                if (k < a.k && s.ids[k] >= 0) {
-                    const float lp = s.p[k] - tmax - logz, p = expf(lp);
-                    const float lq = (zk[u] - top) * invT - lse_t;
-                    if (p != 0.0f) kd += p * (lp - lq);
-                }
+            for (int j = 0; j < P; j++) {
+                e[j] = exp2_hw(__builtin_fmaf(v[j], cT, -mT));
+                st += e[j];
             }
-            kd = group_reduce<W>(kd, Add(), s.buf[3]);
+            if (named) {
+                at_one<P>(pow, e, v, m1, o);
+#pragma unroll
+                for (int j = 0; j < P; j++) s1 += o[j];
+            }
+        });
+        // sum p (log p - (z - top) / T); the log-sum of the student joins when it is known
+        if (taught)
+            for (int k = tid; k < a.k; k += THREADS)
+                if (s.p[k] != 0.0f) kd += s.p[k] * (s.t[k] - __builtin_fmaf(s.z[k], cT, -mT) * LN2);
+        st = wave_reduce(st, Add());
+        if (named) s1 = wave_reduce(s1, Add());
+        if (taught) kd = wave_reduce(kd, Add());
+        if (lane == 0) {
+            s.sum[0][tid >> 6] = st;
+            s.sum[1][tid >> 6] = s1;
+            s.sum[2][tid >> 6] = kd;
         }
+        __syncthreads();
+        st = s1 = kd = 0.0f;
+        for (int w = 0; w < W; w++) {
+            st += s.sum[0][w];
+            s1 += s.sum[1][w];
+            kd += s.sum[2][w];
+        }
+        lse_t = logf(st);
+        lse_1 = named ? logf(s1) : 0.0f;
         if (tid == 0) {
-            float loss = 0.0f;
-            if (taught) loss += wd * a.temperature * a.temperature * kd;
-            if (named) loss += wl * (lse_1 - (zl - top));
+            float loss = 0.0f, psum = 0.0f;
+            if (taught) {
+                // (weights that the exponential rounded to 0 leave the sum at 1, all of them at 0)
+                for (int k = 0; k < a.k && psum == 0.0f; k++) psum += s.p[k];
+                loss = wd * a.temperature * a.temperature * (psum == 0.0f ? 0.0f : kd + lse_t);
+            }
+            if (named) loss += wl * (lse_1 - __builtin_fmaf(zl, LOG2E, -m1) * LN2);
             if (a.loss) a.loss[n] = loss;
             if (a.stats) {
                 a.stats[n * 4] = top;
@@ -225,65 +280,79 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(DistillArgs a)
     // the gradient: q and s from the log-sums, then the entries and the label set again
     const float g = a.drow[n];
     const float gd = g * wd * a.temperature, gl = g * wl;
-    const float bt = lse_t * LOG2E, b1 = lse_1 * LOG2E;
+    const float qd = gd * expf(-lse_t), ql = gl * expf(-lse_1);
+    auto gradients = [&]<int N>(const float *z, float *d) {
+        float o[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) d[j] = exp2_hw(__builtin_fmaf(z[j], cT, -mT));
+        if (named) {
+            at_one<N>(pow, d, z, m1, o);
+#pragma unroll
+            for (int j = 0; j < N; j++) d[j] = qd * d[j] + ql * o[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) d[j] *= qd;
+        }
+    };
     auto base = [&](float z) {
-        float d = 0.0f;
-        if (taught) d = gd * exp2_hw((z - top) * cT - bt);
-        if (named) d += gl * exp2_hw((z - top) * LOG2E - b1);
+        float d;
+        gradients.template operator()<1>(&z, &d);
         return d;
     };
-    each([&](int i, float *v) {
-        float d[P];
+    if (NC > 0 && alike) {
+        const auto to = buffer_from(dbody, sh.pieces * 16);
 #pragma unroll
-        for (int j = 0; j < P; j++) d[j] = base(v[j]);
-        if (alike) dbody[i] = E::pack(d);
-        else
-#pragma unroll
-            for (int j = 0; j < P; j++) E::store(drow, sh.head + i * P + j, d[j]);
-    });
-    if (edge >= 0) E::store(drow, edge, base(zedge));
-    __syncthreads();                     // the row is written: what follows replaces some of it
-#pragma unroll
-    for (int u = 0; u < KPT; u++) {
-        const int k = tid + u * THREADS;
-        if (!taught || k >= a.k || s.ids[k] < 0) continue;
-        // an id that comes more than once is its first entry's to write, with all weights
-        const int id = s.ids[k];
-        float p = 0.0f;
-        bool first = true;
-        for (int j = 0; j < a.k; j++) {
-            if (s.ids[j] != id) continue;
-            if (j < k) first = false;
-            p += expf(s.p[j] - tmax - logz);
+        for (int c = 0; c < NC; c++) {
+            float v[P], d[P];
+            asm volatile("" : "+v"(reg[c]));
+            E::unpack(reg[c], v);
+            gradients.template operator()<P>(v, d);
+            __builtin_amdgcn_raw_buffer_store_b128(E::pack(d), to, tid * 16, c * THREADS * 16, AUX);
         }
-        if (first) E::store(drow, id, base(zk[u]) - gd * p - (named && label == id ? gl : 0.0f));
+    } else {
+        // (the logits are where they were: rows that start otherwise in their 16 bytes are not written in place)
+        for (int i = tid; i < sh.pieces; i += THREADS) {
+            float v[P], d[P];
+            E::unpack(body[i], v);
+            gradients.template operator()<P>(v, d);
+            if (alike) dbody[i] = E::pack(d);
+            else
+#pragma unroll
+                for (int j = 0; j < P; j++) E::store(drow, sh.head + i * P + j, d[j]);
+        }
     }
-    if (named && tid == 0) {
-        bool in = false;
-        if (taught)
-            for (int j = 0; j < a.k; j++) in |= s.ids[j] == (int)label;
-        if (!in) E::store(drow, label, base(zl) - gl);
-    }
+    if (edge >= 0) E::store(drow, edge, base(zedge));
+    const bool listed = __syncthreads_or(label_there);     // (and the row is written: what follows replaces some of it)
+    if (taught)
+        for (int k = tid; k < a.k; k += THREADS)
+            if (!(s.w[k] < 0.0f)) {
+                const int id = s.ids[k];
+                E::store(drow, id, base(s.z[k]) - gd * s.w[k] - (named && label == id ? gl : 0.0f));
+            }
+    if (named && !listed && tid == 0) E::store(drow, label, base(zl) - gl);
 }
 
-template <int DT, int MODE, int THREADS, int NC>
+template <int DT, int MODE, int THREADS, int NC, int WAVES_PER_SIMD, int AUX>
 void go(const DistillArgs &a, hipStream_t stream)
 {
-    distill_kernel<DT, MODE, THREADS, NC><<<(unsigned)a.n, THREADS, 0, stream>>>(a);
+    distill_kernel<DT, MODE, THREADS, NC, WAVES_PER_SIMD, AUX><<<(unsigned)a.n, THREADS, 0, stream>>>(a);
 }
 
-// A row of up to 8 pieces a thread stays in registers (32 of them), with 256 threads for short
-// rows; up to 16 where 1024 threads hold it; longer ones are read again.
+// How many threads hold a row, and how many of its pieces each: as few threads as their registers
+// allow where there are rows for every CU (three rows of 512 threads on a CU, whose loads, sums and
+// stores overlap), 1024 where there are not.
 template <int DT, int MODE>
 void pick(const DistillArgs &a, hipStream_t stream)
 {
     const int64_t pieces = a.vocab / Elem<DT>::PER16 + 1;
-    if (pieces <= 256 * 2) go<DT, MODE, 256, 2>(a, stream);
-    else if (pieces <= 256 * 8) go<DT, MODE, 256, 8>(a, stream);
-    else if (pieces <= 1024 * 4) go<DT, MODE, 1024, 4>(a, stream);
-    else if (pieces <= 1024 * 8) go<DT, MODE, 1024, 8>(a, stream);
-    else if (pieces <= 1024 * 16) go<DT, MODE, 1024, 16>(a, stream);
-    else go<DT, MODE, 1024, 0>(a, stream);
+    const bool few = a.n < 512, big = a.n * pieces * 16 > BIG;
+    if (pieces <= 256 * 2) go<DT, MODE, 256, 2, 6, 0>(a, stream);
+    else if (pieces <= 256 * 8 && !(few && pieces > 1024)) big ? go<DT, MODE, 256, 8, 6, NT>(a, stream) : go<DT, MODE, 256, 8, 6, 0>(a, stream);
+    else if (few && pieces <= 1024 * 4) go<DT, MODE, 1024, 4, 4, 0>(a, stream);
+    else if (few && pieces <= 1024 * 13) go<DT, MODE, 1024, 13, 4, 0>(a, stream);
+    else if (pieces <= 512 * 14) big ? go<DT, MODE, 512, 14, 4, NT>(a, stream) : go<DT, MODE, 512, 14, 4, 0>(a, stream);
+    else if (pieces <= 512 * 25) big ? go<DT, MODE, 512, 25, 2, NT>(a, stream) : go<DT, MODE, 512, 25, 2, 0>(a, stream);
+    else go<DT, MODE, 1024, 0, 4, 0>(a, stream);
 }
 
 template <int MODE>
