@@ -54,7 +54,14 @@ __device__ __forceinline__ f32x16 zero16()
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// The other half-wave's value of the same column, for a maximum or a sum of both.
+template <typename F>
+__device__ __forceinline__ float both_halves(float x, F op)
+{
+    const uint32_t w = __builtin_bit_cast(uint32_t, x);
+    const auto h = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return op(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
 
 // A tile of rows of HD 16-bit elements in LDS, aligned to its rows.  `t` is the tile's offset in LDS.
 typedef __attribute__((address_space(3))) char lds_char;
@@ -311,7 +318,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, s[n][r]);
-        top = fmaxf(top, other_half(top)) * c2;
+        top = both_halves(top, [](float x, float y) { return fmaxf(x, y); }) * c2;
         if (__ballot(top > m)) {
             const float now = fmaxf(m, top);
             const float keep = m == now ? 1.0f : exp2_hw(m - now);     // (both -inf: nothing yet)
@@ -346,7 +353,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
         }
         __syncthreads();
     }
-    l += other_half(l);
+    l = both_halves(l, Add());
     if (!real) return;
     if (a.splits > 1) {
         // unnormalised sums, their maximum and weight, for the join

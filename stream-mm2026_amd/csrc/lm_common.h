@@ -140,14 +140,28 @@ __device__ __forceinline__ void store_any(int dt, void *p, int64_t i, float v)
     else Elem<DT_F16>::store(p, i, v);
 }
 
-// Reductions over a wave: lanes exchange by XOR distance, so every lane ends with the result and
-// the order of the additions is the same on every run.
+// Reductions over a wave without LDS: rotations inside the rows of 16 lanes (DPP), then the rows and
+// the halves swapped.  Lanes only ever combine the same partial results in one order or its mirror,
+// so every lane ends with the same bits, the same ones on every run.
+template <int ROR>
+__device__ __forceinline__ float rotate16(float v)
+{
+    const int i = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, 0x120 + ROR, 0xf, 0xf, false));
+}
 template <typename F>
 __device__ __forceinline__ float wave_reduce(float v, F op)
 {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = op(v, __shfl_xor(v, d, 64));
-    return v;
+    v = op(v, rotate16<8>(v));
+    v = op(v, rotate16<4>(v));
+    v = op(v, rotate16<2>(v));
+    v = op(v, rotate16<1>(v));
+    const uint32_t w = __builtin_bit_cast(uint32_t, v);
+    const auto rows = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    v = op(__uint_as_float(rows[0]), __uint_as_float(rows[1]));
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    const auto halves = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return op(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
 }
 struct Add {
     __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }

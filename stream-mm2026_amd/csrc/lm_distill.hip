@@ -30,6 +30,7 @@ __device__ __forceinline__ int64_t index_at(const void *p, int bytes, int64_t i)
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
 
 // A row's teacher entries: what each thread would otherwise keep in registers over the passes.
 struct RowLds {
@@ -38,7 +39,8 @@ struct RowLds {
     float p[DISTILL_MAX_K];          // weight
     float z[DISTILL_MAX_K];          // the student's logit
     float w[DISTILL_MAX_K];          // the weights of all entries with this id, at its first entry; elsewhere -1
-    float top[16], sum[3][16];
+    float top[16];
+    f32x2 sum[16];
 };
 
 // How a row lies in memory: `head` single elements, `pieces` whole 16-byte pieces, `tail` single ones.
@@ -77,6 +79,17 @@ __device__ __forceinline__ void at_one(int pow, const float *e, const float *z, 
     }
 }
 
+// Values 4 h ... of a piece.
+template <int DT>
+__device__ __forceinline__ void unpack4(u32x4 w, int h, float *v)
+{
+    if constexpr (DT == DT_F32) Elem<DT>::unpack(w, v);
+    else {
+        const f32x2 a = unpack2<DT>(w[2 * h]), b = unpack2<DT>(w[2 * h + 1]);
+        v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1];
+    }
+}
+
 // The memory from p on, `bytes` of it, for buffer accesses (beyond it: zeros read, nothing written).
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_from(const void *p, uint32_t bytes)
 {
@@ -111,17 +124,15 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
     const int edge = tid < sh.head ? tid : tid < sh.head + sh.tail ? vocab - sh.tail + (tid - sh.head) : -1;
     const float zedge = edge >= 0 ? E::load(sh.row, edge) : -__builtin_inff();
 
-    int any = 0;
-    for (int k = tid; k < a.k; k += THREADS) {
+    // whether the row has entries: every wave looks for itself
+    bool any = false;
+    for (int k = lane; k < a.k; k += 64) {
         const int64_t id = index_at(a.ids, a.id_bytes, n * a.k + k);
-        const bool there = id >= 0 && id < vocab;
-        s.ids[k] = there ? (int)id : -1;
-        s.t[k] = there ? load_any(a.teacher_dt, a.teacher, n * a.k + k) * invT : -__builtin_inff();
-        any |= there;
+        any |= id >= 0 && id < vocab;
     }
     const int64_t label = a.labels ? index_at(a.labels, a.label_bytes, n) : -1;
     const bool named = label >= 0 && label < vocab && a.alpha != 1.0f;
-    const bool taught = __syncthreads_or(any) && a.alpha != 0.0f;
+    const bool taught = __any(any) && a.alpha != 0.0f;
     const float wd = taught ? a.alpha : 0.0f, wl = named ? 1.0f - a.alpha : 0.0f;
 
     // dlogits' pieces are those of the logits where both rows start alike in their 16 bytes
@@ -146,58 +157,56 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
         return;
     }
 
-    // the logits at the teacher's entries and the label, read before a gradient may overwrite them
-    for (int k = tid; k < a.k; k += THREADS) s.z[k] = s.ids[k] >= 0 ? E::load(sh.row, s.ids[k]) : 0.0f;
+    // the first wave forms the teacher's distribution, and keeps the logits at its entries, read before a
+    // gradient may overwrite them; the next barrier shows both to the others
     const float zl = named ? E::load(sh.row, label) : 0.0f;
-
-    // the teacher's distribution: its normaliser in every wave, the weights in LDS
-    bool label_there = false;
-    if (taught) {
+    if (taught && tid < 64) {
         float m = -__builtin_inff();
-        for (int k = lane; k < a.k; k += 64) m = Max()(m, s.t[k]);
+        for (int k = lane; k < a.k; k += 64) {
+            const int64_t id = index_at(a.ids, a.id_bytes, n * a.k + k);
+            const bool there = id >= 0 && id < vocab;
+            const float t = there ? load_any(a.teacher_dt, a.teacher, n * a.k + k) * invT : -__builtin_inff();
+            s.ids[k] = there ? (int)id : -1;
+            s.t[k] = t;
+            s.z[k] = there ? E::load(sh.row, id) : 0.0f;
+            m = Max()(m, t);
+        }
         m = wave_reduce(m, Max());
         const float ref = m == -__builtin_inff() ? 0.0f : m;
         float z = 0.0f;
-        for (int k = lane; k < a.k; k += 64) z += expf(s.t[k] - ref);
+        for (int k = lane; k < a.k; k += 64) z += exp2_hw((s.t[k] - ref) * LOG2E);
         z = wave_reduce(z, Add());
-        const float logz = z > 0.0f || z != z ? logf(z) : __builtin_inff();      // every entry at -inf: all weights 0
-        __syncthreads();
-        for (int k = tid; k < a.k; k += THREADS) {
+        const float logz = z > 0.0f || z != z ? log2_hw(z) * LN2 : __builtin_inff();     // every entry at -inf: all weights 0
+        for (int k = lane; k < a.k; k += 64) {
             s.t[k] = s.t[k] - ref - logz;
-            s.p[k] = expf(s.t[k]);
+            s.p[k] = exp2_hw(s.t[k] * LOG2E);
         }
-        __syncthreads();
-        // an id that comes more than once is its first entry's to write, with all weights
-        if (MODE != 0)
-            for (int k = tid; k < a.k; k += THREADS) {
-                const int id = s.ids[k];
-                float w = id < 0 ? -1.0f : 0.0f;
-                if (id >= 0)
-                    for (int j = 0; j < a.k; j++)
-                        if (s.ids[j] == id) w = j < k ? -1.0f : w < 0.0f ? w : w + s.p[j];
-                s.w[k] = w;
-                label_there |= id == (int)label;
-            }
     }
 
     // a value stays packed between its uses: unpacked once and kept, the row would take twice the
     // registers and the CU half the rows
-    auto each = [&](auto f) {            // f(index of the piece, its values)
-        float v[P];
+    auto each = [&](auto f) {            // f(4 values)
+        float v[4];
         if constexpr (NC > 0) {
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-                const int i = tid + c * THREADS;
                 asm volatile("" : "+v"(reg[c]));
-                if (i < sh.pieces) {
-                    E::unpack(reg[c], v);
-                    f(i, v);
+                if (tid + c * THREADS < sh.pieces) {
+#pragma unroll
+                    for (int h = 0; h < P / 4; h++) {
+                        unpack4<DT>(reg[c], h, v);
+                        f(v);
+                    }
                 }
             }
         } else {
             for (int i = tid; i < sh.pieces; i += THREADS) {
-                E::unpack(body[i], v);
-                f(i, v);
+                const u32x4 w = body[i];
+#pragma unroll
+                for (int h = 0; h < P / 4; h++) {
+                    unpack4<DT>(w, h, v);
+                    f(v);
+                }
             }
         }
     };
@@ -205,59 +214,74 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
     // exponents are z c - top c in one rounding; what rounding top c loses is the same for every value
     // of the row and goes out with the sums
     float top, lse_t, lse_1;             // the row's maximum and the two log-sums below it
+    float inv_t, inv_1;                  // 1 / the sums
     if constexpr (MODE == 2) {
         top = a.stats[n * 4];
         lse_t = a.stats[n * 4 + 1];
         lse_1 = a.stats[n * 4 + 2];
+        inv_t = exp2_hw(-lse_t * LOG2E);
+        inv_1 = exp2_hw(-lse_1 * LOG2E);
+        __syncthreads();                 // the teacher's entries
     } else {
         float m = zedge;
-        each([&](int, float *v) {
+        each([&](float *v) {
 #pragma unroll
-            for (int j = 0; j < P; j += 2) m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(v[j], v[j + 1]), m);
+            for (int j = 0; j < 4; j += 2) m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(v[j], v[j + 1]), m);
         });
         top = group_reduce<W>(m, Max(), s.top);
     }
     const float mT = top * cT, m1 = top * LOG2E;
+    // an id that comes more than once is its first entry's to write, with all weights
+    bool label_there = false;
+    if (MODE != 0 && taught)
+        for (int k = tid; k < a.k; k += THREADS) {
+            const int id = s.ids[k];
+            float w = id < 0 ? -1.0f : 0.0f;
+            if (id >= 0)
+                for (int j = 0; j < a.k; j++)
+                    if (s.ids[j] == id) w = j < k ? -1.0f : w < 0.0f ? w : w + s.p[j];
+            s.w[k] = w;
+            label_there |= id == (int)label;
+        }
     if constexpr (MODE != 2) {
         float st = 0.0f, s1 = 0.0f, kd = 0.0f;
         if (edge >= 0) {
             st = exp2_hw(__builtin_fmaf(zedge, cT, -mT));
             if (named) at_one<1>(pow, &st, &zedge, m1, &s1);
         }
-        each([&](int, float *v) {
-            float e[P], o[P];
+        each([&](float *v) {
+            float e[4], o[4];
 #pragma unroll
-            for (int j = 0; j < P; j++) {
+            for (int j = 0; j < 4; j++) {
                 e[j] = exp2_hw(__builtin_fmaf(v[j], cT, -mT));
                 st += e[j];
             }
             if (named) {
-                at_one<P>(pow, e, v, m1, o);
+                at_one<4>(pow, e, v, m1, o);
 #pragma unroll
-                for (int j = 0; j < P; j++) s1 += o[j];
+                for (int j = 0; j < 4; j++) s1 += o[j];
             }
         });
         // sum p (log p - (z - top) / T); the log-sum of the student joins when it is known
-        if (taught)
-            for (int k = tid; k < a.k; k += THREADS)
+        if (taught && tid < 64) {
+            for (int k = lane; k < a.k; k += 64)
                 if (s.p[k] != 0.0f) kd += s.p[k] * (s.t[k] - __builtin_fmaf(s.z[k], cT, -mT) * LN2);
+            kd = wave_reduce(kd, Add());
+        }
         st = wave_reduce(st, Add());
         if (named) s1 = wave_reduce(s1, Add());
-        if (taught) kd = wave_reduce(kd, Add());
-        if (lane == 0) {
-            s.sum[0][tid >> 6] = st;
-            s.sum[1][tid >> 6] = s1;
-            s.sum[2][tid >> 6] = kd;
-        }
+        if (lane == 0) s.sum[tid >> 6] = f32x2{st, s1};
         __syncthreads();
-        st = s1 = kd = 0.0f;
+        st = s1 = 0.0f;
         for (int w = 0; w < W; w++) {
-            st += s.sum[0][w];
-            s1 += s.sum[1][w];
-            kd += s.sum[2][w];
+            const f32x2 t = s.sum[w];
+            st += t[0];
+            s1 += t[1];
         }
-        lse_t = logf(st);
-        lse_1 = named ? logf(s1) : 0.0f;
+        lse_t = log2_hw(st) * LN2;
+        lse_1 = named ? log2_hw(s1) * LN2 : 0.0f;
+        inv_t = 1.0f / st;
+        inv_1 = 1.0f / s1;
         if (tid == 0) {
             float loss = 0.0f, psum = 0.0f;
             if (taught) {
@@ -280,7 +304,7 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
     // the gradient: q and s from the log-sums, then the entries and the label set again
     const float g = a.drow[n];
     const float gd = g * wd * a.temperature, gl = g * wl;
-    const float qd = gd * expf(-lse_t), ql = gl * expf(-lse_1);
+    const float qd = taught ? gd * inv_t : 0.0f, ql = named ? gl * inv_1 : 0.0f;
     auto gradients = [&]<int N>(const float *z, float *d) {
         float o[N];
 #pragma unroll
@@ -299,26 +323,33 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
         gradients.template operator()<1>(&z, &d);
         return d;
     };
+    auto piece = [&](u32x4 w) {
+        float v[4], d[P];
+#pragma unroll
+        for (int h = 0; h < P / 4; h++) {
+            unpack4<DT>(w, h, v);
+            gradients.template operator()<4>(v, d + 4 * h);
+        }
+        return E::pack(d);
+    };
     if (NC > 0 && alike) {
         const auto to = buffer_from(dbody, sh.pieces * 16);
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            float v[P], d[P];
             asm volatile("" : "+v"(reg[c]));
-            E::unpack(reg[c], v);
-            gradients.template operator()<P>(v, d);
-            __builtin_amdgcn_raw_buffer_store_b128(E::pack(d), to, tid * 16, c * THREADS * 16, AUX);
+            __builtin_amdgcn_raw_buffer_store_b128(piece(reg[c]), to, tid * 16, c * THREADS * 16, AUX);
         }
     } else {
         // (the logits are where they were: rows that start otherwise in their 16 bytes are not written in place)
         for (int i = tid; i < sh.pieces; i += THREADS) {
-            float v[P], d[P];
-            E::unpack(body[i], v);
-            gradients.template operator()<P>(v, d);
-            if (alike) dbody[i] = E::pack(d);
-            else
+            const u32x4 w = piece(body[i]);
+            if (alike) dbody[i] = w;
+            else {
+                float d[P];
+                E::unpack(w, d);
 #pragma unroll
                 for (int j = 0; j < P; j++) E::store(drow, sh.head + i * P + j, d[j]);
+            }
         }
     }
     if (edge >= 0) E::store(drow, edge, base(zedge));
@@ -350,8 +381,8 @@ void pick(const DistillArgs &a, hipStream_t stream)
     else if (pieces <= 256 * 8 && !(few && pieces > 1024)) big ? go<DT, MODE, 256, 8, 6, NT>(a, stream) : go<DT, MODE, 256, 8, 6, 0>(a, stream);
     else if (few && pieces <= 1024 * 4) go<DT, MODE, 1024, 4, 4, 0>(a, stream);
     else if (few && pieces <= 1024 * 13) go<DT, MODE, 1024, 13, 4, 0>(a, stream);
-    else if (pieces <= 512 * 14) big ? go<DT, MODE, 512, 14, 4, NT>(a, stream) : go<DT, MODE, 512, 14, 4, 0>(a, stream);
-    else if (pieces <= 512 * 25) big ? go<DT, MODE, 512, 25, 2, NT>(a, stream) : go<DT, MODE, 512, 25, 2, 0>(a, stream);
+    else if (pieces <= 512 * 13) big ? go<DT, MODE, 512, 13, 6, NT>(a, stream) : go<DT, MODE, 512, 13, 6, 0>(a, stream);
+    else if (pieces <= 512 * 25) big ? go<DT, MODE, 512, 25, 4, NT>(a, stream) : go<DT, MODE, 512, 25, 4, 0>(a, stream);
     else go<DT, MODE, 1024, 0, 4, 0>(a, stream);
 }
 

@@ -68,11 +68,8 @@ __device__ __forceinline__ void store_piece(void *p, int64_t row, const Columns<
 template <bool WAVE_ROW>
 __device__ __forceinline__ f32x2 row_sum2(f32x2 v, f32x2 *buf)
 {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        v[0] += __shfl_xor(v[0], d, 64);
-        v[1] += __shfl_xor(v[1], d, 64);
-    }
+    v[0] = wave_reduce(v[0], Add());
+    v[1] = wave_reduce(v[1], Add());
     if constexpr (!WAVE_ROW) {
         if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -85,7 +82,14 @@ __device__ __forceinline__ f32x2 row_sum2(f32x2 v, f32x2 *buf)
 template <bool WAVE_ROW>
 __device__ __forceinline__ float row_sum(float v, f32x2 *buf)
 {
-    return row_sum2<WAVE_ROW>(f32x2{v, 0.0f}, buf)[0];
+    v = wave_reduce(v, Add());
+    if constexpr (!WAVE_ROW) {
+        if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6][0] = v;
+        __syncthreads();
+        v = buf[0][0];
+        for (int w = 1; w < (int)blockDim.x / 64; w++) v += buf[w][0];
+    }
+    return v;
 }
 
 // Mean (layer norms) and 1/deviation of a row in registers: the deviation from the mean itself,
