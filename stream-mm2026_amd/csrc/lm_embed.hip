@@ -214,7 +214,7 @@ __device__ __forceinline__ void finish_row(void *dweight, int64_t at, float *acc
     store_n<DWDT, VEC>(dweight, at, acc);
 }
 
-// Wave w of the grid: entries [SEG w, SEG w + SEG), columns [64 VEC blockIdx.y, ...).  `partial`
+// Wave w of the grid: entries [SEG w, SEG w + SEG), columns [64 VEC blockIdx.x, ...).  `partial`
 // [2 chunks][dim]: a chunk's run that began before it, and the run that goes on behind it.  (A run
 // that does both is the first kind.)
 template <int GDT, int DWDT, int VEC>
@@ -223,29 +223,35 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const int *sorted_tok, c
                                                         int64_t dweight_stride, bool accumulate, float *partial)
 {
     const int lane = threadIdx.x & 63;
-    const int chunk = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int chunk = (blockIdx.y + blockIdx.z * 32768) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = *count;
     const int e0 = chunk * SEG, e1 = min(m, e0 + SEG);
     if (e0 >= m) return;
-    const int col = (blockIdx.y * 64 + lane) * VEC;
+    const int col = (blockIdx.x * 64 + lane) * VEC;
     const bool live = col < dim;
     float acc[VEC] = {};
-    const bool open_front = e0 > 0 && sorted_tok[e0 - 1] == sorted_tok[e0];
-    const bool open_back = e1 < m && sorted_tok[e1] == sorted_tok[e1 - 1];
+    // the chunk's entries, and the tokens on both sides of it (-1: none), one a lane
+    const int at = e0 - 1 + lane;
+    const int toks = lane <= SEG + 1 && at >= 0 && at < m ? sorted_tok[at] : -1;
+    const int poss = lane < SEG && e0 + lane < m ? sorted_pos[e0 + lane] : 0;
+    auto token = [&](int i) { return __builtin_amdgcn_readlane(toks, i + 1); };
+    const int n = e1 - e0;
+    const bool open_front = token(-1) == token(0), open_back = token(n) == token(n - 1);
     bool from_front = open_front;
-    for (int e = e0; e < e1; e += 4) {
-        float g[4][VEC];
+    constexpr int FLY = 8;                         // rows on their way
+    for (int e = 0; e < n; e += FLY) {
+        float g[FLY][VEC];
 #pragma unroll
-        for (int u = 0; u < 4; u++)
-            if (e + u < e1 && live) load_n<GDT, VEC>(grad, (int64_t)sorted_pos[e + u] * grad_stride + col, g[u]);
+        for (int u = 0; u < FLY; u++)
+            if (e + u < n && live) load_n<GDT, VEC>(grad, (int64_t)__builtin_amdgcn_readlane(poss, e + u) * grad_stride + col, g[u]);
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            if (e + u >= e1) break;
-            const int tok = sorted_tok[e + u];
+        for (int u = 0; u < FLY; u++) {
+            if (e + u >= n) break;
+            const int tok = token(e + u);
 #pragma unroll
             for (int k = 0; k < VEC; k++) acc[k] += live ? g[u][k] : 0.0f;
-            const bool at_end = e + u + 1 == e1;
-            if (at_end ? open_back : sorted_tok[e + u + 1] == tok) continue;
+            const bool at_end = e + u + 1 == n;
+            if (at_end ? open_back : token(e + u + 1) == tok) continue;
             // the run of `tok` ends here
             if (live) {
                 if (from_front) store_n<DT_F32, VEC>(partial, (int64_t)(2 * chunk) * dim + col, acc);
@@ -265,23 +271,35 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const int *sorted_tok, 
                                                          int64_t dweight_stride, bool accumulate, const float *partial)
 {
     const int lane = threadIdx.x & 63;
-    const int chunk = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int chunk = (blockIdx.y + blockIdx.z * 32768) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = *count;
     const int e0 = chunk * SEG, e1 = e0 + SEG;
     if (e1 >= m) return;
     const int tok = sorted_tok[e1 - 1];
     if (sorted_tok[e1] != tok || (sorted_tok[e0] == tok && e0 > 0 && sorted_tok[e0 - 1] == tok)) return;
-    const int col = (blockIdx.y * 64 + lane) * VEC;
-    if (col >= dim) return;
-    float acc[VEC];
-    load_n<DT_F32, VEC>(partial, (int64_t)(2 * chunk + 1) * dim + col, acc);
-    // the run's parts: the front of each later chunk that starts with this token
-    for (int c = chunk + 1; (int64_t)c * SEG < m && sorted_tok[c * SEG] == tok; c++) {
-        float v[VEC];
-        load_n<DT_F32, VEC>(partial, (int64_t)(2 * c) * dim + col, v);
+    const int col = (blockIdx.x * 64 + lane) * VEC;
+    const bool live = col < dim;                   // (every lane looks the parts up)
+    float acc[VEC] = {};
+    if (live) load_n<DT_F32, VEC>(partial, (int64_t)(2 * chunk + 1) * dim + col, acc);
+    // the run's parts: the front of each later chunk that starts with this token, 64 looked up at a time
+    for (int c0 = chunk + 1;; c0 += 64) {
+        const int64_t first = (int64_t)(c0 + lane) * SEG;
+        const uint64_t not_mine = ~__ballot(first < m && sorted_tok[first < m ? first : 0] == tok);
+        const int parts = not_mine ? __builtin_ctzll(not_mine) : 64;
+        for (int i = 0; i < parts; i += 8) {
+            float v[8][VEC];
 #pragma unroll
-        for (int k = 0; k < VEC; k++) acc[k] += v[k];
+            for (int u = 0; u < 8; u++)
+                if (i + u < parts && live) load_n<DT_F32, VEC>(partial, (int64_t)(2 * (c0 + i + u)) * dim + col, v[u]);
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                if (i + u < parts)
+#pragma unroll
+                    for (int k = 0; k < VEC; k++) acc[k] += live ? v[u][k] : 0.0f;
+        }
+        if (parts < 64) break;
     }
+    if (!live) return;
     finish_row<DWDT, VEC>(dweight, (int64_t)tok * dweight_stride + col, acc, scale, accumulate);
 }
 
@@ -334,7 +352,9 @@ void launch_bwd(const EmbedArgs &a, const void *grad, int64_t grad_stride, void 
         !accumulate);
     if (a.n == 0) return;
     const int64_t pieces = a.dim / VEC;
-    const dim3 grid((unsigned)((chunks(a.n) + 3) / 4), (unsigned)((pieces + 63) / 64));
+    // (the slices of a chunk's columns side by side: their rows' lines are neighbours in memory)
+    const int64_t wgs = (chunks(a.n) + 3) / 4;
+    const dim3 grid((unsigned)((pieces + 63) / 64), (unsigned)(wgs < 32768 ? wgs : 32768), (unsigned)((wgs + 32767) / 32768));
     embed_sum_kernel<GDT, DWDT, VEC><<<grid, 256, 0, stream>>>(tok, pos, count, grad, grad_stride, (int)a.dim, a.scale, dweight,
                                                                dweight_stride, accumulate, partial);
     if (a.n > SEG)

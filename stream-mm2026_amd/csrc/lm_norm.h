@@ -28,14 +28,15 @@ struct NormArgs {
     float *workspace;
 };
 
-// How the backward pass's workgroups share the rows: with few groups of gates `per_group`
-// workgroups to a group; with many (per_group 0) each worker takes whole groups.
+// How the rows are shared out.  `waves` a row (1 and 2: several rows of a workgroup of four waves;
+// more: a workgroup's).  Backward: with few groups of gates `per_group` workgroups to a group, with
+// many (per_group 0) each row's threads take whole groups.
 struct NormSplit {
-    int wgs, per_group;
+    int wgs, per_group, waves, fwd_wgs;
 };
 
-// The row kernels of one element type (lm_norm_f32.hip, lm_norm_bf16.hip, lm_norm_f16.hip).
-template <int DT>
+// The row kernels of one element type, with weights of that type or fp32 (lm_norm_*.hip).
+template <int DT, bool WF32>
 hipError_t norm_run(const NormArgs &a, const NormSplit &sp, bool ragged, bool backward, hipStream_t stream);
 
 hipError_t norm_forward(const NormArgs &a, hipStream_t stream);

@@ -6,7 +6,9 @@
 namespace lm {
 namespace {
 
-constexpr int MAX_WGS = 512;       // workgroups of the backward pass (its partial rows)
+// Workgroups of the backward pass (each leaves a partial row) and of the forward pass: as many waves as
+// the chip holds of each (16 a CU).
+int most_wgs(int waves) { return waves <= 4 ? 1024 : waves <= 8 ? 512 : 256; }
 
 // Adds the partial rows: blockIdx.y names the sum (4 and up: the groups of the gate).  64 columns a
 // workgroup, its 16 waves take every 16th partial row.
@@ -27,6 +29,7 @@ __global__ __launch_bounds__(1024) void norm_finish_kernel(NormArgs a, NormSplit
     float s = 0.0f;
     if (col < a.dim) {
         const float *p = a.workspace + (which * (int64_t)sp.wgs + first) * a.dim + col;
+#pragma unroll 8
         for (int64_t r = wave; r < rows; r += 16) s += p[r * a.dim];
     }
     buf[wave][lane] = s;
@@ -41,16 +44,23 @@ int size_of(int dt) { return dt == DT_F32 ? 4 : 2; }
 
 NormSplit split_of(int64_t n, int64_t dim, int64_t groups)
 {
-    const int workers = dim <= 1024 ? 4 : 1;
-    if (groups <= MAX_WGS) {
-        const int64_t rpg = n / groups;
-        int64_t per = MAX_WGS / groups, most = (rpg + workers - 1) / workers;
-        if (per > most) per = most;
-        if (per < 1) per = 1;
-        return {(int)(groups * per), (int)per};
+    NormSplit s;
+    const int64_t waves = (dim + 511) / 512;
+    s.waves = (int)waves;
+    const int rows = waves == 1 ? 4 : waves == 2 ? 2 : 1, most = most_wgs(s.waves);
+    s.fwd_wgs = most;
+    s.per_group = 0;
+    if (groups <= most) {
+        const int64_t rpg = n / groups, each = (rpg + rows - 1) / rows;
+        int64_t per = most / groups;
+        if (per > each) per = each;
+        s.per_group = (int)(per < 1 ? 1 : per);
+        s.wgs = (int)groups * s.per_group;
+    } else {
+        const int64_t wgs = (groups + rows - 1) / rows;
+        s.wgs = (int)(wgs < most ? wgs : most);
     }
-    const int64_t wgs = (groups + workers - 1) / workers;
-    return {(int)(wgs < MAX_WGS ? wgs : MAX_WGS), 0};
+    return s;
 }
 
 // Whether every row of every array can be read and written 16 bytes at a time.
@@ -70,13 +80,15 @@ bool wide(const NormArgs &a, bool backward)
 hipError_t by_type(const NormArgs &a, bool backward, hipStream_t stream)
 {
     // (without rows the sums of no partial rows are written: zeros)
-    const NormSplit sp = a.n ? split_of(a.n, a.dim, a.groups) : NormSplit{0, 0};
+    const NormSplit sp = a.n ? split_of(a.n, a.dim, a.groups) : NormSplit{0, 0, 0, 0};
     const bool ragged = !wide(a, backward);
     hipError_t e = hipSuccess;
     if (a.n)
-        e = a.dt == DT_F32    ? norm_run<DT_F32>(a, sp, ragged, backward, stream)
-            : a.dt == DT_BF16 ? norm_run<DT_BF16>(a, sp, ragged, backward, stream)
-                              : norm_run<DT_F16>(a, sp, ragged, backward, stream);
+        e = a.dt == DT_F32                  ? norm_run<DT_F32, true>(a, sp, ragged, backward, stream)
+            : a.dt == DT_BF16 && a.weight_dt ? norm_run<DT_BF16, false>(a, sp, ragged, backward, stream)
+            : a.dt == DT_BF16                ? norm_run<DT_BF16, true>(a, sp, ragged, backward, stream)
+            : a.weight_dt                    ? norm_run<DT_F16, false>(a, sp, ragged, backward, stream)
+                                             : norm_run<DT_F16, true>(a, sp, ragged, backward, stream);
     if (e != hipSuccess || !backward) return e;
     const unsigned sums = a.gate && (sp.per_group || !a.n) ? 4 + (unsigned)a.groups : 4;
     norm_finish_kernel<<<dim3((unsigned)((a.dim + 63) / 64), sums), 1024, 0, stream>>>(a, sp);

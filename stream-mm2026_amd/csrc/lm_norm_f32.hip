@@ -2,5 +2,5 @@
 #include "lm_norm_kernel.h"
 
 namespace lm {
-template hipError_t norm_run<DT_F32>(const NormArgs &, const NormSplit &, bool, bool, hipStream_t);
+template hipError_t norm_run<DT_F32, true>(const NormArgs &, const NormSplit &, bool, bool, hipStream_t);
 }
