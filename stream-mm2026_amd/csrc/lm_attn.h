@@ -35,14 +35,18 @@ constexpr int MAX_SPLITS = 512;
 int attn_splits(const AttnArgs &a);
 int64_t attn_forward_workspace(const AttnArgs &a);
 
-// Where the work on the keys' gradients is cut: blocks of 128 keys, and for the first `sink_blocks` of
-// them `far` more shares of `step` positions each, which lie behind the window of the block's keys.
+// Where the work on the keys' gradients is cut: blocks of 128 keys, and either (few blocks) the walk of
+// each over its positions in `shares` parts, or (sinks) for the first `sink_blocks` of them `far` more
+// workgroups of `step` positions each, which lie behind the window of the block's keys.
 struct DkvSplit {
-    int blocks, sink_blocks, far, step;
-    // The partial sums of share f (0: the blocks' own): dk and dv of the sinks.
+    int blocks, sink_blocks, far, step, shares;
+    __host__ __device__ int parts() const { return shares > 1 ? shares : far + 1; }
+    // the keys whose gradients come in parts
+    __host__ __device__ int keys(const AttnArgs &a) const { return shares > 1 ? a.keys : far ? a.sinks : 0; }
+    // the partial sums of part f: dk and dv of those keys
     __host__ __device__ float *sums(const AttnArgs &a, int head, int f) const
     {
-        return a.partial + ((int64_t)head * (far + 1) + f) * 2 * a.sinks * a.dim;
+        return a.partial + ((int64_t)head * parts() + f) * 2 * keys(a) * a.dim;
     }
 };
 DkvSplit dkv_split(const AttnArgs &a);

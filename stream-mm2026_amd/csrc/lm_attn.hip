@@ -29,12 +29,26 @@ int64_t attn_forward_workspace(const AttnArgs &a)
 // its window go to workgroups of their own.  Sinks that fill many blocks need none of this.
 DkvSplit dkv_split(const AttnArgs &a)
 {
-    DkvSplit s = {(a.keys + 127) / 128, (a.sinks + 127) / 128, 0, 1};
+    DkvSplit s = {(a.keys + 127) / 128, (a.sinks + 127) / 128, 0, 1, 1};
+    // fewer workgroups than the chip holds: their walks in parts, of four tiles of 32 rows at least
+    const int64_t wgs = (int64_t)a.batch * a.key_heads * s.blocks;
+    if (wgs < 384 && a.rows) {
+        const int64_t walk = (int64_t)(a.window + 127 < a.keys && a.sinks == 0 ? a.window + 127 : a.keys) * a.group / 32;
+        int64_t shares = 512 / wgs;
+        if (shares > walk / 4) shares = walk / 4;
+        if (shares > 16) shares = 16;
+        if (shares > 1) {
+            s.shares = (int)shares;
+            return s;
+        }
+    }
     const int64_t behind = (int64_t)a.keys - (127 + a.window);                // positions that see the sinks alone
     const int64_t others = (int64_t)a.batch * a.key_heads * s.blocks * (a.window + 128);
     if (a.sinks == 0 || a.sinks > 256 || behind < 512 || others > 3 * 256 * (int64_t)a.keys) return s;
-    s.step = a.window > 512 ? a.window : 512;
-    if (s.step < behind / 16) s.step = (int)(behind / 16);
+    // shares of an eighth of a block's own walk: they are launched last and fill the gaps (as long as the
+    // walk itself, 24 of them behind 512 blocks doubled the time)
+    s.step = (a.window + 127) / 8 > 128 ? (a.window + 127) / 8 : 128;
+    if (s.step < behind / 32) s.step = (int)(behind / 32);
     s.far = (int)((behind + s.step - 1) / s.step);
     return s;
 }
@@ -44,7 +58,7 @@ int64_t attn_backward_delta(const AttnArgs &a) { return ((int64_t)a.batch * a.he
 int64_t attn_backward_workspace(const AttnArgs &a)
 {
     const DkvSplit s = dkv_split(a);
-    const int64_t sums = s.far ? (int64_t)a.batch * a.key_heads * (s.far + 1) * 2 * a.sinks * a.dim : 0;
+    const int64_t sums = (int64_t)a.batch * a.key_heads * s.parts() * 2 * s.keys(a) * a.dim;
     return attn_backward_delta(a) + sums;
 }
 

@@ -618,9 +618,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
     lds_char *const lds = (lds_char *)lds_;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
-    // blockIdx.y: the blocks of keys, then the sinks' far positions
-    const int far = (int)blockIdx.y < cut.blocks ? -1 : ((int)blockIdx.y - cut.blocks) % cut.far;
-    const int block = far < 0 ? blockIdx.y : (blockIdx.y - cut.blocks) / cut.far;
+    // blockIdx.y: the blocks of keys, then their other parts: of the walk, or the sinks' far positions
+    const int y = blockIdx.y, more = y - cut.blocks;
+    const int share = cut.shares > 1 ? y / cut.blocks : 0;
+    const int far = cut.shares > 1 || more < 0 ? -1 : more % cut.far;
+    const int block = far >= 0 ? more / cut.far : y - share * cut.blocks;
     const int k0 = block * WAVES * 32, ka = k0 + wave * 32, key = ka + (lane & 31);
     const Sight sight = {a.window, a.sinks};
     const int before = a.keys - a.rows;
@@ -661,6 +663,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
         p0 = max(near + far * cut.step, before);
         p1 = min(a.keys, near + (far + 1) * cut.step);
     } else if (k0 < a.sinks && cut.far == 0) p1 = a.keys;
+    if (cut.shares > 1) {
+        const int each = (max(0, p1 - p0) + cut.shares - 1) / cut.shares;
+        p0 += share * each;
+        p1 = min(p1, p0 + each);
+    }
     const int first = (p0 - before) * a.group, last = (p1 - before) * a.group;      // rows
     S qs, gs;
     float lse_r = 0.0f, delta_r = 0.0f;
@@ -671,34 +678,52 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
     // and `rest` heads on)
     int t0 = p0 - before, over = 0, row_in = first;
     const int whole_t = 32 / a.group, rest = 32 - whole_t * a.group;
-    auto fetch = [&]() {
-        const auto qr = buffer_from(qp + t0 * a.q.t), gr = buffer_from(gp + t0 * a.dout.t);
-        uint32_t qo[S::N], go[S::N];
+    // where the thread's pieces of a tile and its row's statistics lie, from position t0 on: the same for
+    // every tile where the heads that share a key head divide 32
+    uint32_t qo[S::N], go[S::N];
+    int stat_r = 0, stat_t = 0;
+    auto place = [&]() {
 #pragma unroll
         for (int i = 0; i < S::N; i++) {
             // small numbers, divided in fp32
             const int r = over + S::row() + i * S::STEP, t = (int)(((float)r + 0.5f) * per_group), g = r - t * a.group;
-            const bool there = row_in + S::row() + i * S::STEP < last && S::piece() * 8 < a.dim;
+            const bool there = S::piece() * 8 < a.dim;
             qo[i] = there ? (t * (uint32_t)a.q.t + g * (uint32_t)a.q.h + S::piece() * 8) * 2 : NOWHERE;
             go[i] = there ? (t * (uint32_t)a.dout.t + g * (uint32_t)a.dout.h + S::piece() * 8) * 2 : NOWHERE;
         }
-        qs.load(qr, [&](int i) { return qo[i]; });
-        gs.load(gr, [&](int i) { return go[i]; });
+        const int r = over + (threadIdx.x & 31);
+        stat_t = (int)(((float)r + 0.5f) * per_group);
+        stat_r = (r - stat_t * a.group) * a.rows + stat_t;
+    };
+    place();
+    const int64_t stat0 = ((int64_t)b * a.heads + hk * a.group) * a.rows;
+    auto fetch = [&]() {
+        const auto qr = buffer_from(qp + t0 * a.q.t), gr = buffer_from(gp + t0 * a.dout.t);
+        if (row_in + 32 <= last) {
+            qs.load(qr, [&](int i) { return qo[i]; });
+            gs.load(gr, [&](int i) { return go[i]; });
+        } else {
+            auto there = [&](int i) { return row_in + S::row() + i * S::STEP < last; };
+            qs.load(qr, [&](int i) { return there(i) ? qo[i] : NOWHERE; });
+            gs.load(gr, [&](int i) { return there(i) ? go[i] : NOWHERE; });
+        }
         if (threadIdx.x < 32) {                          // (looked at when the tile is stored)
-            const int r = over + min((int)threadIdx.x, last - 1 - row_in), t = (int)(((float)r + 0.5f) * per_group), g = r - t * a.group;
-            const int64_t stat = ((int64_t)b * a.heads + hk * a.group + g) * a.rows + t0 + t;
-            lse_r = a.lse[stat];
-            delta_r = a.delta[stat];
-            pos_r = before + t0 + t;
-            // behind the last row there is no weight
-            if (row_in + (int)threadIdx.x >= last) pos_r = -1;
+            pos_r = -1;                                  // behind the last row there is no weight
+            if (row_in + (int)threadIdx.x < last) {
+                lse_r = a.lse[stat0 + t0 + stat_r];
+                delta_r = a.delta[stat0 + t0 + stat_r];
+                pos_r = before + t0 + stat_t;
+            }
         }
         row_in += 32;
         t0 += whole_t;
-        over += rest;
-        if (over >= a.group) {
-            over -= a.group;
-            t0++;
+        if (rest) {
+            over += rest;
+            if (over >= a.group) {
+                over -= a.group;
+                t0++;
+            }
+            place();
         }
     };
     auto store = [&](int side) {
@@ -773,8 +798,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
         __syncthreads();
     }
     if (!real) return;
-    if (cut.far && key < a.sinks) {
-        float *part = cut.sums(a, blockIdx.x, far + 1) + key * a.dim;
+    const int part_keys = cut.keys(a);
+    if (key < part_keys) {
+        float *part = cut.sums(a, blockIdx.x, share + far + 1) + (int64_t)key * a.dim;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -782,7 +808,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
                 const int e = 32 * d + result_row(r, lane);
                 if (e >= a.dim) continue;
                 *(f32x4 *)(part + e) = f32x4{dk[d][r], dk[d][r + 1], dk[d][r + 2], dk[d][r + 3]};
-                *(f32x4 *)(part + a.sinks * a.dim + e) = f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
+                *(f32x4 *)(part + (int64_t)part_keys * a.dim + e) = f32x4{dv[d][r], dv[d][r + 1], dv[d][r + 2], dv[d][r + 3]};
             }
         return;
     }
@@ -800,18 +826,20 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
         }
 }
 
-// Adds the partial sums of the sinks: a thread 2 elements of one key.
+// Adds the parts of dk and dv: a thread 2 elements of one key.
 template <int DT>
-__global__ __launch_bounds__(256) void attn_sinks_kernel(AttnArgs a, DkvSplit cut)
+__global__ __launch_bounds__(256) void attn_parts_kernel(AttnArgs a, DkvSplit cut)
 {
-    const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
+    const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads, keys = cut.keys(a), parts = cut.parts();
     const int i = blockIdx.y * 256 + threadIdx.x, key = i / (a.dim / 2), e = i % (a.dim / 2) * 2;
-    if (key >= a.sinks) return;
+    if (key >= keys) return;
+    const float *part = cut.sums(a, blockIdx.x, 0) + (int64_t)key * a.dim + e;
+    const int64_t other = (int64_t)keys * a.dim;
     f32x2 k = {0.0f, 0.0f}, v = {0.0f, 0.0f};
-    for (int f = 0; f <= cut.far; f++) {
-        const float *part = cut.sums(a, blockIdx.x, f) + key * a.dim + e;
+#pragma unroll 4
+    for (int f = 0; f < parts; f++, part += 2 * other) {
         k += *(const f32x2 *)part;
-        v += *(const f32x2 *)(part + a.sinks * a.dim);
+        v += *(const f32x2 *)(part + other);
     }
     *(uint32_t *)((uint16_t *)at(a.dk, b, hk) + (int64_t)key * a.dk.t + e) = pack2<DT>(k[0] * a.scale, k[1] * a.scale);
     *(uint32_t *)((uint16_t *)at(a.dv, b, hk) + (int64_t)key * a.dv.t + e) = pack2<DT>(v[0], v[1]);
@@ -836,8 +864,8 @@ void run_backward(const AttnArgs &a, hipStream_t stream)
     const int64_t rows = (int64_t)a.batch * a.heads * a.rows;
     const DkvSplit cut = dkv_split(a);
     if (rows) attn_delta_kernel<DT><<<(unsigned)((rows + 31) / 32), 256, 0, stream>>>(a);
-    attn_dkv_kernel<DT, HD, 4><<<dim3(heads, cut.blocks + cut.sink_blocks * cut.far), 256, 0, stream>>>(a, cut);
-    if (cut.far) attn_sinks_kernel<DT><<<dim3(heads, (a.sinks * a.dim / 2 + 255) / 256), 256, 0, stream>>>(a, cut);
+    attn_dkv_kernel<DT, HD, 4><<<dim3(heads, cut.blocks * cut.shares + cut.sink_blocks * cut.far), 256, 0, stream>>>(a, cut);
+    if (cut.parts() > 1) attn_parts_kernel<DT><<<dim3(heads, (unsigned)(((int64_t)cut.keys(a) * a.dim / 2 + 255) / 256)), 256, 0, stream>>>(a, cut);
     if (rows) attn_dq_kernel<DT, HD, 4><<<dim3(heads, (total + 127) / 128), 256, 0, stream>>>(a);
 }
 
