@@ -101,7 +101,9 @@ typedef struct stq_tensor4 {
  * and sees key j <= p if p - j < window (window 0: no limit) or j < sinks, and key_mask[batch, j] is
  * nonzero.  A row that sees nothing gives zeros, and zero gradients; what masked keys hold does not
  * matter.  BFloat16 or Half; dim a multiple of 8 up to 128; heads a multiple of key_heads, consecutive
- * heads sharing one; scale > 0.  Pointers are 16-byte aligned, strides multiples of 8.
+ * heads sharing one; scale 1e-30 to 1e30.  Pointers are 16-byte aligned, strides multiples of 8.
+ * Limits: keys and rows * (heads / key_heads) up to 2^22, batch * key_heads up to 65535, row_stride 0 to
+ * 2^22, head_stride >= 0 and of q and dout, times heads / key_heads, up to 2^29.
  * out is rounded once; softmax weights are rounded to dtype before the products with them.
  * lse: [batch, heads, rows] floats, written forward, read backward.
  */
@@ -130,7 +132,7 @@ int stq_attention_backward(const stq_attention *a, void *stream);
  * An entry whose id lies outside [0, vocab) is absent, a label outside it or a null `labels` too; a
  * row without entries has no first term, one without label no second, and one with neither is 0.
  * logits, dlogits: [n, vocab] of one type, rows strided; dlogits may be logits itself.  teacher, ids:
- * [n, k] dense, 0 <= k <= 1024.  loss: [n] floats or null.  stats: [n, 4] floats.
+ * [n, k] dense, 0 <= k <= 1024.  temperature: 1e-15 to 1e15; alpha: 0 to 1.  loss: [n] floats or null.  stats: [n, 4] floats.
  * forward: dlogits null: loss and stats; dlogits given: loss and dlogits from one read of the logits.
  * backward: dlogits from the stats of a forward call.
  */

@@ -248,7 +248,12 @@ struct KeyStage {
 __device__ __forceinline__ const uint16_t *at(const AttnTensor &t, int b, int h) { return (const uint16_t *)t.p + b * t.b + h * t.h; }
 
 // ---------------------------------------------------------------- forward
-// WAVES x 32 rows; the keys in tiles of 64, or the share of them that blockIdx.z takes.
+// WAVES x 32 rows; the keys in tiles of 64, or the share of them that blockIdx.z takes.  Bound by the waves'
+// issue: per score two products of the head size against one exponential and about six vector instructions,
+// so most of a tile's cycles are the softmax's.  A maximum that does not grow skips the rescaling.  Tiles of
+// up to 32 rows run as one wave, where latency counts.  Window 2048 with 4 sinks over 8192 positions, 32
+// heads of 128 on 8 of keys, bf16: 305-333 us, 0.8 PFLOP/s of visible products; 12 heads of 64, 8 x 1024
+// causal: 31 us.
 template <int DT, int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void attn_fwd_kernel(AttnArgs a)
 {
@@ -300,51 +305,50 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
         const lds_char *kt = lds + turn, *vt = kt + BYTES;
         asm volatile("" : "+v"(rp), "+v"(cp));     // the reads' addresses are formed where they are used, not kept
         if (see != 0 && !sight.none(pa, pb, key, key + TILE - 1)) {
-
-        f32x16 s[2] = {zero16(), zero16()};
-#pragma unroll
-        for (int c = 0; c < C; c++)
-#pragma unroll
-            for (int n = 0; n < 2; n++) s[n] = mma<DT>(Tile<HD>::rows(kt, rp, 32 * n, c), q[c], s[n]);
-        if (see != ~0ull || !sight.all(pa, pb, key, key + TILE - 1)) {
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const uint32_t bits = visible16(sight, pos, key + 32 * n, (uint32_t)(see >> (32 * n)), lane);
-                hide(s[n], bits);
+            f32x16 s[2] = {zero16(), zero16()};
+    #pragma unroll
+            for (int c = 0; c < C; c++)
+    #pragma unroll
+                for (int n = 0; n < 2; n++) s[n] = mma<DT>(Tile<HD>::rows(kt, rp, 32 * n, c), q[c], s[n]);
+            if (see != ~0ull || !sight.all(pa, pb, key, key + TILE - 1)) {
+    #pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const uint32_t bits = visible16(sight, pos, key + 32 * n, (uint32_t)(see >> (32 * n)), lane);
+                    hide(s[n], bits);
+                }
             }
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) top = fmaxf(top, s[n][r]);
-        top = both_halves(top, [](float x, float y) { return fmaxf(x, y); }) * c2;
-        if (__ballot(top > m)) {
-            const float now = fmaxf(m, top);
-            const float keep = m == now ? 1.0f : exp2_hw(m - now);     // (both -inf: nothing yet)
-            m = now;
-            l *= keep;
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) o[d][r] *= keep;
-        }
-        const float ref = m == -__builtin_inff() ? 0.0f : m;
-#pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                s[n][r] = exp2_hw(__builtin_fmaf(s[n][r], c2, -ref));
-                l += s[n][r];
+            float top = s[0][0];
+    #pragma unroll
+            for (int n = 0; n < 2; n++)
+    #pragma unroll
+                for (int r = 0; r < 16; r++) top = fmaxf(top, s[n][r]);
+            top = both_halves(top, [](float x, float y) { return fmaxf(x, y); }) * c2;
+            if (__ballot(top > m)) {
+                const float now = fmaxf(m, top);
+                const float keep = m == now ? 1.0f : exp2_hw(m - now);     // (both -inf: nothing yet)
+                m = now;
+                l *= keep;
+    #pragma unroll
+                for (int d = 0; d < ND; d++)
+    #pragma unroll
+                    for (int r = 0; r < 16; r++) o[d][r] *= keep;
             }
-#pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const u32x4 p = operand<DT>(s[n], 8 * k);
-#pragma unroll
-                for (int d = 0; d < ND; d++) o[d] = mma<DT>(Tile<HD>::columns(vt, cp, 32 * n + 16 * k, d), p, o[d]);
-            }
+            const float ref = m == -__builtin_inff() ? 0.0f : m;
+    #pragma unroll
+            for (int n = 0; n < 2; n++)
+    #pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[n][r] = exp2_hw(__builtin_fmaf(s[n][r], c2, -ref));
+                    l += s[n][r];
+                }
+    #pragma unroll
+            for (int n = 0; n < 2; n++)
+    #pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const u32x4 p = operand<DT>(s[n], 8 * k);
+    #pragma unroll
+                    for (int d = 0; d < ND; d++) o[d] = mma<DT>(Tile<HD>::columns(vt, cp, 32 * n + 16 * k, d), p, o[d]);
+                }
         }
         turn ^= 2 * BYTES;
         if (it + 1 < it1) {
@@ -497,7 +501,10 @@ __device__ __forceinline__ void settle(f32x16 &ds, const f32x16 &p, uint32_t vis
     for (int r = 0; r < 16; r++) ds[r] = (visible >> r & 1) && !(p[r] > 1.0f - 0x1p-16f) ? ds[r] : 0.0f;
 }
 
-// dq of WAVES x 32 rows: the forward pass's walk over the keys.
+// dq of WAVES x 32 rows: the forward pass's walk over the keys, 32 keys at a time so that scores, their
+// gradients and the sums fit the registers of two waves a SIMD.  Three products a score; the walk that is
+// shared with dk and dv would save two of their seven and need atomic sums of dq, whose order changes
+// results.  The forward's window of 2048: 385-415 us; 8 x 12 x 1024 of 64: 37 us.
 template <int DT, int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a)
 {
@@ -554,32 +561,32 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
         const lds_char *kt = lds + turn, *vt = kt + BYTES;
         asm volatile("" : "+v"(rp), "+v"(cp));     // the reads' addresses are formed where they are used, not kept
         if (see != 0 && !sight.none(pa, pb, key, key + TILE - 1)) {
-        const bool whole = see == ~0ull && sight.all(pa, pb, key, key + TILE - 1);
-        for (int n = 0; n < 2; n++) {
-            uint32_t bits = 0;                           // which of the lane's 16 results are visible
-            if (!whole) bits = visible16(sight, pos, key + 32 * n, (uint32_t)(see >> (32 * n)), lane);
-            __builtin_amdgcn_sched_barrier(0);
-            f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-            for (int c = 0; c < C; c++) {
-                s = mma<DT>(Tile<HD>::rows(kt + n * (32 * Tile<HD>::ROW), rp, 0, c), q[c], s);
-                dp = mma<DT>(Tile<HD>::rows(vt + n * (32 * Tile<HD>::ROW), rp, 0, c), g[c], dp);
+            const bool whole = see == ~0ull && sight.all(pa, pb, key, key + TILE - 1);
+            for (int n = 0; n < 2; n++) {
+                uint32_t bits = 0;                           // which of the lane's 16 results are visible
+                if (!whole) bits = visible16(sight, pos, key + 32 * n, (uint32_t)(see >> (32 * n)), lane);
+                __builtin_amdgcn_sched_barrier(0);
+                f32x16 s = zero16(), dp = zero16();
+    #pragma unroll
+                for (int c = 0; c < C; c++) {
+                    s = mma<DT>(Tile<HD>::rows(kt + n * (32 * Tile<HD>::ROW), rp, 0, c), q[c], s);
+                    dp = mma<DT>(Tile<HD>::rows(vt + n * (32 * Tile<HD>::ROW), rp, 0, c), g[c], dp);
+                }
+                if (!whole) hide(s, bits);
+    #pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[r] = exp2_hw(__builtin_fmaf(s[r], c2, -lse));
+                    dp[r] = s[r] * (dp[r] - delta);
+                }
+                if (!whole) settle(dp, s, bits);
+                __builtin_amdgcn_sched_barrier(0);
+    #pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const u32x4 p = operand<DT>(dp, 8 * k);
+    #pragma unroll
+                    for (int d = 0; d < ND; d++) dq[d] = mma<DT>(Tile<HD>::columns(kt + n * (32 * Tile<HD>::ROW), cp, 16 * k, d), p, dq[d]);
+                }
             }
-            if (!whole) hide(s, bits);
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                s[r] = exp2_hw(__builtin_fmaf(s[r], c2, -lse));
-                dp[r] = s[r] * (dp[r] - delta);
-            }
-            if (!whole) settle(dp, s, bits);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const u32x4 p = operand<DT>(dp, 8 * k);
-#pragma unroll
-                for (int d = 0; d < ND; d++) dq[d] = mma<DT>(Tile<HD>::columns(kt + n * (32 * Tile<HD>::ROW), cp, 16 * k, d), p, dq[d]);
-            }
-        }
         }
         turn ^= 2 * BYTES;
         if (it + 1 < tiles.count) {
@@ -603,7 +610,11 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
 
 // dk and dv of WAVES x 32 keys: over the rows that see any of them, 32 at a time.  A workgroup takes the
 // positions whose window holds a key of its block; those behind that, which see the sinks alone, go to
-// workgroups of their own (DkvSplit), whose sums are fp32 partial results.
+// workgroups of their own, and where there are few blocks each one's walk is cut into shares (DkvSplit);
+// the sums are fp32 partial results then.  Four products a score.  Heads of 128 hold k in registers and v
+// in LDS (both in registers spilled; separate kernels for dk and dv formed the scores twice and were slower
+// together).  The forward's window of 2048: 611 us, with the sinks' far positions in their block's own walk
+// 900; ragged fp16 sequences of few blocks 43 us and 7 to add their parts, in one walk each 109.
 template <int DT, int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, DkvSplit cut)
 {
@@ -750,43 +761,43 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
         const lds_char *qt = lds + side * 2 * BYTES, *gt = qt + BYTES;
         asm volatile("" : "+v"(rp), "+v"(cp));     // the reads' addresses are formed where they are used, not kept
         if (!sight.none(pa, pb, ka, ka + 31)) {
-        const bool whole = all_seen && sight.all(pa, pb, ka, ka + 31);
-        uint32_t bits = 0;                               // which of the lane's 16 results are visible
-        if (!whole) {
+            const bool whole = all_seen && sight.all(pa, pb, ka, ka + 31);
+            uint32_t bits = 0;                               // which of the lane's 16 results are visible
+            if (!whole) {
+                for (int r = 0; r < 16; r += 4) {
+                    const u32x4 po = *(const u32x4 *)(pos_s[side] + result_row(r, lane));
+    #pragma unroll
+                    for (int k = 0; k < 4; k++) bits |= (uint32_t)(seen && sight.one((int)po[k], key)) << (r + k);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            f32x16 s = zero16(), dp = zero16();
+    #pragma unroll
+            for (int c = 0; c < C; c++) {
+                s = mma<DT>(Tile<HD>::rows(qt, rp, 0, c), kf[c], s);
+                dp = mma<DT>(Tile<HD>::rows(gt, rp, 0, c), values(c), dp);
+            }
+            if (!whole) hide(s, bits);
+    #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const u32x4 po = *(const u32x4 *)(pos_s[side] + result_row(r, lane));
-#pragma unroll
-                for (int k = 0; k < 4; k++) bits |= (uint32_t)(seen && sight.one((int)po[k], key)) << (r + k);
+                const f32x4 ls = *(const f32x4 *)(lse_s[side] + result_row(r, lane)), de = *(const f32x4 *)(delta_s[side] + result_row(r, lane));
+    #pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    s[r + k] = exp2_hw(__builtin_fmaf(s[r + k], c2, -ls[k]));
+                    dp[r + k] = s[r + k] * (dp[r + k] - de[k]);
+                }
             }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            s = mma<DT>(Tile<HD>::rows(qt, rp, 0, c), kf[c], s);
-            dp = mma<DT>(Tile<HD>::rows(gt, rp, 0, c), values(c), dp);
-        }
-        if (!whole) hide(s, bits);
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const f32x4 ls = *(const f32x4 *)(lse_s[side] + result_row(r, lane)), de = *(const f32x4 *)(delta_s[side] + result_row(r, lane));
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                s[r + k] = exp2_hw(__builtin_fmaf(s[r + k], c2, -ls[k]));
-                dp[r + k] = s[r + k] * (dp[r + k] - de[k]);
+            if (!whole) settle(dp, s, bits);
+            __builtin_amdgcn_sched_barrier(0);
+    #pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const u32x4 p = operand<DT>(s, 8 * k), ds = operand<DT>(dp, 8 * k);
+    #pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    dv[d] = mma<DT>(Tile<HD>::columns(gt, cp, 16 * k, d), p, dv[d]);
+                    dk[d] = mma<DT>(Tile<HD>::columns(qt, cp, 16 * k, d), ds, dk[d]);
+                }
             }
-        }
-        if (!whole) settle(dp, s, bits);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const u32x4 p = operand<DT>(s, 8 * k), ds = operand<DT>(dp, 8 * k);
-#pragma unroll
-            for (int d = 0; d < ND; d++) {
-                dv[d] = mma<DT>(Tile<HD>::columns(gt, cp, 16 * k, d), p, dv[d]);
-                dk[d] = mma<DT>(Tile<HD>::columns(qt, cp, 16 * k, d), ds, dk[d]);
-            }
-        }
         }
         side ^= 1;
         pa = pb;

@@ -190,7 +190,8 @@ int check_attention_sizes(const stq_attention *a)
 int check_attention(const stq_attention *a, bool backward)
 {
     CHECK(check_attention_sizes(a));
-    if (!(a->scale > 0.0) || !std::isfinite(a->scale)) return bad("scale must be finite and > 0");
+    // (a float of 0 would turn hidden scores, -inf, into NaN, an infinite one scores of 0)
+    if (!(a->scale >= 1e-30 && a->scale <= 1e30)) return bad("scale must be finite and > 0 (1e-30 to 1e30)");
     if (a->batch == 0 || a->keys == 0 || (a->rows == 0 && !backward)) return STQ_OK;
     const int64_t group = a->heads / a->key_heads;
     if (a->rows && (group * a->q.head_stride > 1 << 29 || (backward && group * a->dout.head_stride > 1 << 29)))
@@ -255,7 +256,8 @@ int check_distill(const stq_distill *a)
     CHECK(check_size("n", a->n, 0, INT_MAX));
     CHECK(check_size("vocab", a->vocab, 1, 1 << 30));
     CHECK(check_size("teacher entries", a->k, 0, lm::DISTILL_MAX_K));
-    if (!(a->temperature > 0.0) || !std::isfinite(a->temperature)) return bad("temperature must be finite and > 0");
+    // (its square and its reciprocal are floats)
+    if (!(a->temperature >= 1e-15 && a->temperature <= 1e15)) return bad("temperature must be finite and > 0 (1e-15 to 1e15)");
     if (!(a->alpha >= 0.0 && a->alpha <= 1.0)) return bad("alpha must be 0 to 1");
     if (a->n == 0) return STQ_OK;
     CHECK(check_ptr("logits", a->logits, size_of(a->dtype)));

@@ -15,6 +15,8 @@
 //      tokens in registers.  A run inside its entries is final; the parts of a run that crosses
 //      the border go to fp32 partial rows.
 //   3. join: the wave that holds a crossing run's first entry adds its parts in order.
+// The gradient of 8192 tokens over 50257 x 768: 24-30 us for the sort and 48 MB of zeros, 12 and 4 us for
+// the rest; of 32768 tokens that favour few: 34, 60 and 7 us.
 #include "lm_common.h"
 #include "lm_embed.h"
 
@@ -32,7 +34,9 @@ __device__ __forceinline__ int64_t token_at(const void *tokens, int bytes, int64
 }
 
 // ---------------------------------------------------------------- lookup
-// A workgroup takes whole rows, about 1024 pieces of VEC elements (blockIdx.y cuts longer rows).
+// A workgroup takes whole rows, about 1024 pieces of VEC elements (blockIdx.y cuts longer rows): four
+// independent 16-byte loads a thread in flight.  8192 rows of 768 bf16: 10 us; 32768 rows of 1024 fp32 to
+// bf16 from a vocabulary that favours few tokens: 48 us, 4.2 TB/s of what is read and written.
 template <int WDT, int ODT, int VEC>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const void *tokens, int token_bytes, int64_t n, int64_t vocab, int dim,
                                                         float scale, const void *weight, int64_t weight_stride, void *out,
@@ -72,8 +76,8 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void *tokens, int 
 // ---------------------------------------------------------------- sort
 struct SortLds {
     int hist[SORT_WAVES][MAX_RANGE];              // counts, then each wave's next place
-    uint32_t list[SORT_WAVES][LIST];              // local token in the high 9 bits of ...
-    uint32_t pos[SORT_WAVES][LIST];
+    uint32_t list[SORT_WAVES][LIST];              // the first entries of each wave: token less the range's first,
+    uint32_t pos[SORT_WAVES][LIST];               // and position
     int wave_sum[SORT_WAVES];
     int below[SORT_WAVES];
 };

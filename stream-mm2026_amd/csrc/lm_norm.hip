@@ -11,7 +11,7 @@ namespace {
 int most_wgs(int waves) { return waves <= 4 ? 1024 : waves <= 8 ? 512 : 256; }
 
 // Adds the partial rows: blockIdx.y names the sum (4 and up: the groups of the gate).  64 columns a
-// workgroup, its 16 waves take every 16th partial row.
+// workgroup, its 16 waves take every 16th partial row.  1024 partial rows of 768 4.5 us, 512 of 4096 9.4 us.
 __global__ __launch_bounds__(1024) void norm_finish_kernel(NormArgs a, NormSplit sp)
 {
     __shared__ float buf[16][64];

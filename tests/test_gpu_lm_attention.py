@@ -174,6 +174,22 @@ def test_split_keys(b, h, hk, t, s, d):
     check(q, k, v, do, window=700, sinks=130)
 
 
+@pytest.mark.parametrize("b,h,hk,t,s,d,dtype", [(1, 7, 1, 1100, 1100, 64, BF16), (1, 2, 2, 700, 1500, 128, F16), (2, 40, 2, 70, 600, 72, BF16)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 0), (150, 130), (40, 3)])
+def test_gradients_of_few_blocks_of_keys(b, h, hk, t, s, d, dtype, window, sinks):
+    """Walks in shares, some of them without a row; a batch with masked keys."""
+    mask = torch.rand(b, s, device="cuda", generator=ref.gen(s)) < 0.8
+    check(*inputs(t + window, b, h, hk, t, s, d, dtype), window=window, sinks=sinks, key_mask=mask)
+
+
+@pytest.mark.parametrize("d,group,window,sinks", [(64, 1, 64, 3), (128, 1, 100, 200), (64, 3, 1, 1), (128, 2, 300, 128)])
+def test_gradients_of_sinks_seen_from_far(d, group, window, sinks):
+    """Many blocks of keys: the positions that see the sinks alone are workgroups of their own."""
+    mask = torch.ones(4, 1600, dtype=torch.bool, device="cuda")
+    mask[1, :2], mask[2, 1:900] = False, False
+    check(*inputs(d + window, 4, 8 * group, 8, 1600, 1600, d, BF16), window=window, sinks=sinks, key_mask=mask)
+
+
 def test_autograd_and_differences():
     q, k, v, do = inputs(8, 2, 4, 2, 60, 60, 64, BF16)
     leaf = [x.clone().requires_grad_(True) for x in (q, k, v)]

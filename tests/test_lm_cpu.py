@@ -157,6 +157,26 @@ def test_attention_refusals(backward, kw, msg):
 DISTILL = dict(n=4, v=100, dt=1, z=P, zs=100, t=P, tdt=0, ids=P, idt=9, k=5, lab=0, ldt=9, temp=1.0, alpha=0.5, loss=P, stats=P, drow=P, dz=0, dzs=0)
 
 
+@pytest.mark.parametrize("backward,kw,msg", [
+    (False, dict(scale=1e-40), "scale must be finite and > 0"),        # a float of 0
+    (False, dict(scale=1e39), "scale must be finite and > 0"),         # an infinite float
+    (False, dict(t4=dict(k=(P, 2048, 512, (1 << 22) + 8))), "k: row_stride must be 0 to 2^22"),
+    (False, dict(t4=dict(v=(P, 2048, -8, 64))), "v: row_stride must be 0 to 2^22, head_stride >= 0"),
+    (False, dict(t4=dict(q=(P, 2048, (1 << 28) + 8, 64))), "q and dout: the heads of a key head must lie within 2^29"),
+    (True, dict(t4=dict(dout=(P, 2048, (1 << 28) + 8, 64))), "q and dout: the heads of a key head must lie within 2^29"),
+    (False, dict(b=40000), "batch * key_heads must be 0 to 65535"),
+    (False, dict(t=8, s=(1 << 22) + 1), "keys must be 0 to"),
+    (False, dict(t=(1 << 21) + 1, s=1 << 22), "rows * heads / key_heads must be 0 to"),
+])
+def test_attention_limits(backward, kw, msg):
+    assert attention(backward, **kw) == INVALID and msg in err()
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e-16, 1e16, 1e39])
+def test_distill_temperatures_outside_the_floats(temperature):
+    assert distill(temp=temperature) == INVALID and "temperature must be finite and > 0" in err()
+
+
 def distill(backward=False, **kw):
     L = _capi.lm_lib()
     return (L.stq_distill_backward if backward else L.stq_distill_forward)(lm._DISTILL.pack(*(DISTILL | kw).values()), None)
