@@ -106,6 +106,22 @@ __device__ __forceinline__ u32x4 operand(const f32x16 &s, int r0)
                  pack2<DT>(s[r0 + 6], s[r0 + 7])};
 }
 
+// What that rounding left, as an operand of its own.  Rows that see few keys have the largest score
+// gradients, and the tiles in which they see them are not all visible: only there dS is multiplied as
+// two parts (dq of 8 x 12 x 1024 of 64: 1.49 times the error of a product in fp32 before, 1.35 now, for
+// 2 us of 37).
+template <int DT>
+__device__ __forceinline__ u32x4 remainder(const f32x16 &s, int r0, u32x4 rounded)
+{
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const f32x2 x = unpack2<DT>(rounded[i]);
+        o[i] = pack2<DT>(s[r0 + 2 * i] - x[0], s[r0 + 2 * i + 1] - x[1]);
+    }
+    return o;
+}
+
 // Waits for loaded registers here.  Loads that are first used inside a loop are otherwise waited for
 // there, on every turn, and with them the loop's own loads for its next turn.
 template <int N>
@@ -504,7 +520,7 @@ __device__ __forceinline__ void settle(f32x16 &ds, const f32x16 &p, uint32_t vis
 // dq of WAVES x 32 rows: the forward pass's walk over the keys, 32 keys at a time so that scores, their
 // gradients and the sums fit the registers of two waves a SIMD.  Three products a score; the walk that is
 // shared with dk and dv would save two of their seven and need atomic sums of dq, whose order changes
-// results.  The forward's window of 2048: 385-415 us; 8 x 12 x 1024 of 64: 37 us.
+// results.  The forward's window of 2048: 414-443 us; 8 x 12 x 1024 of 64: 38 us.
 template <int DT, int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a)
 {
@@ -585,6 +601,11 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
                     const u32x4 p = operand<DT>(dp, 8 * k);
     #pragma unroll
                     for (int d = 0; d < ND; d++) dq[d] = mma<DT>(Tile<HD>::columns(kt + n * (32 * Tile<HD>::ROW), cp, 16 * k, d), p, dq[d]);
+                    if (!whole) {
+                        const u32x4 rest = remainder<DT>(dp, 8 * k, p);
+#pragma unroll
+                        for (int d = 0; d < ND; d++) dq[d] = mma<DT>(Tile<HD>::columns(kt + n * (32 * Tile<HD>::ROW), cp, 16 * k, d), rest, dq[d]);
+                    }
                 }
             }
         }
@@ -614,7 +635,7 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
 // the sums are fp32 partial results then.  Four products a score.  Heads of 128 hold k in registers and v
 // in LDS (both in registers spilled; separate kernels for dk and dv formed the scores twice and were slower
 // together).  The forward's window of 2048: 611 us, with the sinks' far positions in their block's own walk
-// 900; ragged fp16 sequences of few blocks 43 us and 7 to add their parts, in one walk each 109.
+// 900; ragged fp16 sequences of few blocks 45 us and 7 to add their parts, in one walk each 109.
 template <int DT, int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, DkvSplit cut)
 {
@@ -796,6 +817,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
                 for (int d = 0; d < ND; d++) {
                     dv[d] = mma<DT>(Tile<HD>::columns(gt, cp, 16 * k, d), p, dv[d]);
                     dk[d] = mma<DT>(Tile<HD>::columns(qt, cp, 16 * k, d), ds, dk[d]);
+                }
+                if (!whole) {
+                    const u32x4 rest = remainder<DT>(dp, 8 * k, ds);
+#pragma unroll
+                    for (int d = 0; d < ND; d++) dk[d] = mma<DT>(Tile<HD>::columns(qt, cp, 16 * k, d), rest, dk[d]);
                 }
             }
         }

@@ -373,7 +373,7 @@ void go(const DistillArgs &a, hipStream_t stream)
 // How many threads hold a row, and how many of its pieces each.  With rows for every CU, few threads with
 // many registers: three rows of 512 threads and 13 pieces run on a CU, whose loads, sums and stores overlap
 // (8192 rows of 50257: 375 us; two of 14 pieces 425).  With fewer than two rows a CU, 1024 threads, which
-// bring one row in sooner (16 rows of 50257: loss and gradient 13 us).
+// bring one row in sooner (7 rows of 32000 fp32: loss 6.0 us, its gradient 6.8 us).
 template <int DT, int MODE>
 void pick(const DistillArgs &a, hipStream_t stream)
 {
