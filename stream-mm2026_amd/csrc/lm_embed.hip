@@ -15,7 +15,7 @@
 //      tokens in registers.  A run inside its entries is final; the parts of a run that crosses
 //      the border go to fp32 partial rows.
 //   3. join: the wave that holds a crossing run's first entry adds its parts in order.
-// The gradient of 8192 tokens over 50257 x 768: 24-30 us for the sort and 48 MB of zeros, 12 and 4 us for
+// The gradient of 8192 tokens over 50257 x 768: 24-30 us for the sort and 131 MB of zeros, 12 and 4 us for
 // the rest; of 16384 tokens that favour few over 32000 x 4096 bf16: 34, 60 and 7 us.
 #include "lm_common.h"
 #include "lm_embed.h"
