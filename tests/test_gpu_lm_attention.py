@@ -229,3 +229,25 @@ def test_the_same_bits_every_time_on_any_stream_and_in_a_graph():
         torch.cuda.synchronize()
         o2, l2 = lm.attention_forward(q, k, v, **kw)
         assert torch.equal(out, o2) and all(torch.equal(a, b) for a, b in zip(grads, lm.attention_backward(do, q, k, v, o2, l2, **kw))), step
+
+
+@pytest.mark.parametrize("t,s,window,sinks,masked", [(3, 3, 0, 0, False), (16, 16, 0, 0, False), (17, 17, 0, 0, False), (200, 200, 9, 4, False),
+                                                     (200, 200, 16, 1, False), (300, 300, 0, 0, True), (300, 300, 150, 3, True)])
+@pytest.mark.parametrize("h,hk,d,dtype", [(4, 2, 64, BF16), (3, 1, 128, F16), (5, 5, 24, BF16)])
+def test_rows_of_few_keys_need_no_exact_output(t, s, window, sinks, masked, h, hk, d, dtype):
+    """A row of up to 16 keys takes delta from its weights: its dq is the same bits whatever ``out`` holds, and the
+    other rows' delta follows ``out``."""
+    q, k, v, do = inputs(t + d, 2, h, hk, t, s, d, dtype)
+    mask = None
+    if masked:
+        mask = torch.rand(2, s, device="cuda", generator=ref.gen(t)) < 0.5
+        mask[1, :260] = False
+    kw = dict(window=window, sinks=sinks, key_mask=mask)
+    out, lse, dq, _, _ = check(q, k, v, do, **kw)
+    other, _, _ = lm.attention_backward(do, q, k, v, out + 1, lse, **kw)
+    count = ref.visible(t, s, window, sinks, mask, 2, "cuda").sum(-1)
+    few = count <= 16
+    same = (dq == other).all(-1).transpose(1, 2)              # [batch, position, head]
+    assert bool(same[few].all())
+    if bool((~few).any()):
+        assert not bool(same[~few].all())
