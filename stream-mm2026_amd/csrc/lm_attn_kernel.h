@@ -122,6 +122,44 @@ __device__ __forceinline__ u32x4 remainder(const f32x16 &s, int r0, u32x4 rounde
     return o;
 }
 
+// fp16 holds fewer bits below 2^-14, and a score gradient is about |dout| / keys: rounded as it is, dq of 4500
+// keys with dout of 1e-3 was off by 0.5 % (0.07 % is its own rounding).  Each column is therefore multiplied by a
+// power of two that keeps its largest score gradient so far within 2^13 .. 2^15, and the sums with it; the power
+// goes out of them at the end.  Like a running maximum it is looked at every tile and seldom changes.  bfloat16
+// has the exponents of fp32 and needs none of this.
+template <int DT>
+struct Lift {
+    static constexpr bool ON = DT == DT_F16;
+    float up = ON ? 0x1p60f : 1.0f;                // down to dout's and the weights' smallest; no float overflows
+
+    template <int ND>
+    __device__ __forceinline__ void fit(f32x16 &ds, f32x16 (&sums)[ND])
+    {
+        if constexpr (ON) {
+            float top = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                ds[r] *= up;
+                top = fmaxf(top, fabsf(ds[r]));
+            }
+            top = both_halves(top, [](float x, float y) { return fmaxf(x, y); });
+            if (__ballot(top > 0x1p15f)) {
+                // (an infinite one stays what it is)
+                const bool over = top > 0x1p15f && top < __builtin_inff();
+                const float by = over ? __builtin_ldexpf(1.0f, 14 - __builtin_amdgcn_frexp_expf(top)) : 1.0f;
+                up *= by;
+#pragma unroll
+                for (int r = 0; r < 16; r++) ds[r] *= by;
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) sums[d][r] *= by;
+            }
+        }
+    }
+    __device__ __forceinline__ float down() const { return 1.0f / up; }      // (exact: a power of two)
+};
+
 // Waits for loaded registers here.  Loads that are first used inside a loop are otherwise waited for
 // there, on every turn, and with them the loop's own loads for its next turn.
 template <int N>
@@ -619,6 +657,7 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
 #pragma unroll
     for (int d = 0; d < ND; d++) dq[d] = zero16();
     const float c2 = a.scale * LOG2E;
+    Lift<DT> lift;
     KeyStage<HD, WAVES * 64> next;
     int rp = Tile<HD>::row_place(lane), cp = Tile<HD>::column_place(lane);
     uint64_t see = 0;
@@ -650,6 +689,7 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
                     dp[r] = s[r] * (dp[r] - delta);
                 }
                 if (!whole) settle(dp, s, bits);
+                lift.fit(dp, dq);
                 __builtin_amdgcn_sched_barrier(0);
     #pragma unroll
                 for (int k = 0; k < 2; k++) {
@@ -672,6 +712,7 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
         __syncthreads();
     }
     if (!real) return;
+    const float scale = a.scale * lift.down();
     uint16_t *po = (uint16_t *)at(a.dq, b, head) + t * a.dq.t;
 #pragma unroll
     for (int d = 0; d < ND; d++)
@@ -679,8 +720,8 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
         for (int r = 0; r < 16; r += 4) {
             const int e = 32 * d + result_row(r, lane);
             if (e < a.dim)
-                *(u32x2 *)(po + e) = u32x2{pack2<DT>(dq[d][r] * a.scale, dq[d][r + 1] * a.scale),
-                                           pack2<DT>(dq[d][r + 2] * a.scale, dq[d][r + 3] * a.scale)};
+                *(u32x2 *)(po + e) = u32x2{pack2<DT>(dq[d][r] * scale, dq[d][r + 1] * scale),
+                                           pack2<DT>(dq[d][r + 2] * scale, dq[d][r + 3] * scale)};
         }
 }
 
@@ -742,6 +783,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
 #pragma unroll
     for (int d = 0; d < ND; d++) dk[d] = dv[d] = zero16();
     const float c2 = a.scale * LOG2E;
+    Lift<DT> lift;
     // the positions that see a key of this workgroup: [p0, p1)
     const int k1 = min(a.keys, k0 + WAVES * 32) - 1;
     const int near = min(a.keys, k1 + a.window);
@@ -864,6 +906,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
                 }
             }
             if (!whole) settle(dp, s, bits);
+            lift.fit(dp, dk);
             __builtin_amdgcn_sched_barrier(0);
     #pragma unroll
             for (int k = 0; k < 2; k++) {
@@ -890,6 +933,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
         __syncthreads();
     }
     if (!real) return;
+    if constexpr (Lift<DT>::ON) {
+        const float down = lift.down();
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) dk[d][r] *= down;
+    }
     const int part_keys = cut.keys(a);
     if (key < part_keys) {
         float *part = cut.sums(a, blockIdx.x, share + far + 1) + (int64_t)key * a.dim;
