@@ -528,8 +528,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a)
 // delta = rowsum(dout * out): 16 lanes a row.  A row that sees up to FEW_KEYS keys takes sum P (do v^T) from
 // them instead: `out` is rounded, and what that puts into delta falls with the number of keys, while the
 // rounding of dS does not (a handful of positions: the error of dq 1.05 times that of products in fp32, 2.3
-// before; 8 x 12 x 1024 of 64 11 us, 6 before; a wave a row in turn 38).
+// before; 8 x 12 x 1024 of 64 11 us, 6 before; a wave a row in turn 38).  It is divided by the sum of the same
+// weights, which lse's rounding leaves off 1: a weight of 1 - 2^-17 beside one of 2^-17 keeps its gradient.  A row
+// that sees one key has no score gradient at all: its delta says LONE.
 constexpr int FEW_KEYS = 16;
+constexpr uint32_t LONE = 0x7fc01e01u;             // a NaN of these bits
+__device__ __forceinline__ bool is_lone(float delta) { return __builtin_bit_cast(uint32_t, delta) == LONE; }
+
 template <int DT>
 __global__ __launch_bounds__(256, 6) void attn_delta_kernel(AttnArgs a)
 {
@@ -593,21 +598,25 @@ __global__ __launch_bounds__(256, 6) void attn_delta_kernel(AttnArgs a)
 #pragma unroll
             for (int e = 0; e < 8; e++) dp += x[e] * y[e];
         }
-        float de = mine ? exp2_hw(__builtin_fmaf(sc, a.scale * LOG2E, -lse * LOG2E)) * dp : 0.0f;
+        float p = mine ? exp2_hw(__builtin_fmaf(sc, a.scale * LOG2E, -lse * LOG2E)) : 0.0f;
+        float de = mine ? p * dp : 0.0f;
 #pragma unroll
-        for (int d = 8; d; d >>= 1) de += __shfl_xor(de, d, 64);
-        if (few) s = de;
+        for (int d = 8; d; d >>= 1) {
+            p += __shfl_xor(p, d, 64);
+            de += __shfl_xor(de, d, 64);
+        }
+        if (few) s = p == 0.0f ? 0.0f : de / p;
+        if (few && count == 1 && fabsf(lse) < __builtin_inff()) s = __builtin_bit_cast(float, LONE);
     }
     if (row < total && part == 0) a.delta[stat] = s;
 }
 
-// A weight of all but 2^-16 leaves its row's other keys less than the rounding of `out` puts into
-// delta: the softmax is constant there and dS is 0 (exactly so where a row sees one key).  A row
-// that sees that few keys meets them in tiles that are not all visible, the only ones to ask.
-__device__ __forceinline__ void settle(f32x16 &ds, const f32x16 &p, uint32_t visible)
+// Scores that are hidden have no gradient, nor have those of LONE rows: their bits in `live` are 0.  Such rows
+// meet their key in tiles that are not all visible, the only ones to ask.
+__device__ __forceinline__ void settle(f32x16 &ds, uint32_t live)
 {
 #pragma unroll
-    for (int r = 0; r < 16; r++) ds[r] = (visible >> r & 1) && !(p[r] > 1.0f - 0x1p-16f) ? ds[r] : 0.0f;
+    for (int r = 0; r < 16; r++) ds[r] = (live >> r & 1) ? ds[r] : 0.0f;
 }
 
 // dq of WAVES x 32 rows: the forward pass's walk over the keys, 32 keys at a time so that scores, their
@@ -688,7 +697,7 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
                     s[r] = exp2_hw(__builtin_fmaf(s[r], c2, -lse));
                     dp[r] = s[r] * (dp[r] - delta);
                 }
-                if (!whole) settle(dp, s, bits);
+                if (!whole) settle(dp, is_lone(delta) ? 0 : bits);
                 lift.fit(dp, dq);
                 __builtin_amdgcn_sched_barrier(0);
     #pragma unroll
@@ -880,13 +889,18 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
         asm volatile("" : "+v"(rp), "+v"(cp));     // the reads' addresses are formed where they are used, not kept
         if (!sight.none(pa, pb, ka, ka + 31)) {
             const bool whole = all_seen && sight.all(pa, pb, ka, ka + 31);
-            uint32_t bits = 0;                               // which of the lane's 16 results are visible
+            uint32_t bits = 0, live = 0;                     // which of the lane's 16 results are visible; not LONE
             if (!whole) {
                 for (int r = 0; r < 16; r += 4) {
                     const u32x4 po = *(const u32x4 *)(pos_s[side] + result_row(r, lane));
+                    const f32x4 de = *(const f32x4 *)(delta_s[side] + result_row(r, lane));
     #pragma unroll
-                    for (int k = 0; k < 4; k++) bits |= (uint32_t)(seen && sight.one((int)po[k], key)) << (r + k);
+                    for (int k = 0; k < 4; k++) {
+                        bits |= (uint32_t)(seen && sight.one((int)po[k], key)) << (r + k);
+                        live |= (uint32_t)!is_lone(de[k]) << (r + k);
+                    }
                 }
+                live &= bits;
             }
             __builtin_amdgcn_sched_barrier(0);
             f32x16 s = zero16(), dp = zero16();
@@ -905,7 +919,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
                     dp[r + k] = s[r + k] * (dp[r + k] - de[k]);
                 }
             }
-            if (!whole) settle(dp, s, bits);
+            if (!whole) settle(dp, live);
             lift.fit(dp, dk);
             __builtin_amdgcn_sched_barrier(0);
     #pragma unroll
