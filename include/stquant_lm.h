@@ -105,7 +105,7 @@ typedef struct stq_tensor4 {
  * Limits: keys and rows * (heads / key_heads) up to 2^22, batch * key_heads up to 65535, row_stride 0 to
  * 2^22, head_stride >= 0 and of q and dout, times heads / key_heads, up to 2^29.
  * out is rounded once; softmax weights and the gradients of the scores are rounded to dtype before the
- * products with them (the latter of Half times a power of two that keeps them among its normal numbers).
+ * products with them (those of Half times a power of two that keeps them among its normal numbers).
  * lse: [batch, heads, rows] floats, written forward, read backward.
  */
 typedef struct stq_attention {

@@ -106,6 +106,12 @@ __device__ __forceinline__ u32x4 operand(const f32x16 &s, int r0)
                  pack2<DT>(s[r0 + 6], s[r0 + 7])};
 }
 
+// The weights of fp16 are multiplied by 2^14 before they are rounded, which the sums give back: they are at most 1,
+// and over n keys about 1 / n, of which fp16 holds ever fewer bits below 2^-14 (dv of 200,000 keys: off by 0.20 %,
+// 0.02 % so).
+template <int DT>
+constexpr float RAISE = DT == DT_F16 ? 14.0f : 0.0f;
+
 // What that rounding left, as an operand of its own.  Rows that see few keys have the largest score
 // gradients, and the tiles in which they see them are not all visible: only there dS is multiplied as
 // two parts (dq of 8 x 12 x 1024 of 64: 1.49 times the error of a product in fp32 before, 1.35 now, for
@@ -342,7 +348,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
     f32x16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = zero16();
-    float m = -__builtin_inff(), l = 0.0f;         // in units of log2; l of this lane's keys alone
+    float m = -__builtin_inff(), l = 0.0f;         // in units of log2; l of this lane's keys alone, and raised
     const float c2 = a.scale * LOG2E;
     KeyStage<HD, WAVES * 64> next;
     int rp = Tile<HD>::row_place(lane), cp = Tile<HD>::column_place(lane);
@@ -387,14 +393,16 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
     #pragma unroll
                     for (int r = 0; r < 16; r++) o[d][r] *= keep;
             }
-            const float ref = m == -__builtin_inff() ? 0.0f : m;
+            const float ref = (m == -__builtin_inff() ? 0.0f : m) - RAISE<DT>;
+            float sum = 0.0f;              // (added to l once a tile: beside a large l single weights would be lost)
     #pragma unroll
             for (int n = 0; n < 2; n++)
     #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     s[n][r] = exp2_hw(__builtin_fmaf(s[n][r], c2, -ref));
-                    l += s[n][r];
+                    sum += s[n][r];
                 }
+            l += sum;
     #pragma unroll
             for (int n = 0; n < 2; n++)
     #pragma unroll
@@ -412,6 +420,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
         __syncthreads();
     }
     l = both_halves(l, Add());
+    m -= RAISE<DT>;                                // what the sums stand against
     if (!real) return;
     if (a.splits > 1) {
         // unnormalised sums, their maximum and weight, for the join
@@ -869,7 +878,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
         gs.store(lds + side * 2 * BYTES + BYTES);
         if (threadIdx.x < 32) {
             const bool none = pos_r < 0 || lse_r == -__builtin_inff();   // nor where a row sees nothing
-            lse_s[side][threadIdx.x] = none ? __builtin_inff() : lse_r * LOG2E;
+            lse_s[side][threadIdx.x] = none ? __builtin_inff() : __builtin_fmaf(lse_r, LOG2E, -RAISE<DT>);
             delta_s[side][threadIdx.x] = none ? 0.0f : delta_r;
             pos_s[side][threadIdx.x] = pos_r;
         }
@@ -948,11 +957,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
     }
     if (!real) return;
     if constexpr (Lift<DT>::ON) {
-        const float down = lift.down();
+        const float back = __builtin_ldexpf(1.0f, -(int)RAISE<DT>), down = lift.down() * back;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) dk[d][r] *= down;
+            for (int r = 0; r < 16; r++) {
+                dk[d][r] *= down;
+                dv[d][r] *= back;
+            }
     }
     const int part_keys = cut.keys(a);
     if (key < part_keys) {

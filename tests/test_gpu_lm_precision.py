@@ -87,3 +87,65 @@ def test_a_row_of_one_key_has_no_score_gradient_at_any_score():
             out, lse = lm.attention_forward(q, k, v, scale=scale, key_mask=mask)
             dq, dk, dv = lm.attention_backward(do, q, k, v, out, lse, scale=scale, key_mask=mask)
             assert not bool(dq.any()) and not bool(dk.any()) and bool(dv.any())
+
+
+@pytest.mark.parametrize("t,s,window", [(200, 200, 0), (70, 300, 90)])
+@pytest.mark.parametrize("h,hk,d,dtype", [(2, 2, 64, BF16), (4, 2, 128, F16)])
+@pytest.mark.parametrize("scale", [3.0, 9.0])
+def test_gradients_of_scores_in_the_hundreds(t, s, window, h, hk, d, dtype, scale):
+    """Peaked rows, |lse| of hundreds: the weights carry fp32's error of the scores and of lse, 2^-22 of their magnitudes."""
+    g = ref.gen(t + d)
+    q, do = (ref.randn(g, 1, h, t, d, dtype=dtype) for _ in range(2))
+    k, v = (ref.randn(g, 1, hk, s, d, dtype=dtype) for _ in range(2))
+    kw = dict(window=window, scale=scale)
+    out, lse = lm.attention_forward(q, k, v, **kw)
+    got = lm.attention_backward(do, q, k, v, out, lse, **kw)
+    want = ref.attention_with_bounds(q, k, v, do, **kw)
+    e = 2.0 ** -22 * scale * float((q.double().abs() @ k.double().abs().repeat_interleave(h // hk, 1).transpose(-1, -2).contiguous()).max())
+    _, wl, p = ref.attention(q, k, v, **kw)
+    assert float(wl.abs().max()) > 60 and float(p.amax(-1).median()) > 0.9
+    kk, vv = (x.double().repeat_interleave(h // hk, 1) for x in (k, v))
+    dp = do.double() @ vv.transpose(-1, -2).contiguous()
+    # (weights below fp32's and bfloat16's smallest normal number are 0, and score gradients too)
+    see = ref.visible(t, s, window, 0, None, 1, "cuda")[:, None]
+    eds = 2 * e * p * scale * (dp.abs() + (p * dp.abs()).sum(-1, keepdim=True)) + see * 2.0 ** -125 * scale * (1 + dp.abs() + dp.abs().amax(-1, keepdim=True))
+    tr = lambda x: x.transpose(-1, -2).contiguous()  # noqa: E731
+    shared = lambda x: x.reshape(1, hk, h // hk, s, d).sum(2)  # noqa: E731
+    more = {"dq": eds @ kk.abs(), "dk": shared(tr(eds) @ q.double().abs()), "dv": shared(tr(2 * e * p + see * 2.0 ** -125) @ do.double().abs())}
+    assert bool(got[0].any()) and bool(got[1].any())
+    for name, x in zip(("dq", "dk", "dv"), got):
+        ref.within(name, x, want[name][0], want[name][1] + more[name])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_fp16_weights_of_long_contexts_keep_their_bits(d):
+    """Normalised weights over 200,000 keys are 2^-18 on average, below fp16's full precision (2^-14): one rounding of
+    them in dv."""
+    g = ref.gen(d)
+    q, do = ref.randn(g, 1, 1, 64, d, dtype=F16), ref.randn(g, 1, 1, 64, d, std=100.0, dtype=F16)
+    k, v = (ref.randn(g, 1, 1, 200_000, d, dtype=F16) for _ in range(2))
+    out, lse = lm.attention_forward(q, k, v)
+    dv = lm.attention_backward(do, q, k, v, out, lse)[2]
+    _, wl, p = ref.attention(q, k, v)
+    near("dv", dv, p.transpose(-1, -2).contiguous() @ do.double(), 1)
+    assert float((lse.double() - wl).abs().max()) <= 2.0 ** -17 * (1 + float(wl.abs().max()))
+
+
+def test_fp16_a_key_far_above_many():
+    """A first key 17 above 2^20 others: each of those weighs e^-17, 0.7 of fp16's smallest number, together 4 %.
+
+    The weights' rounding, alike for all of them, and the sum's of 16,384 tiles, 2^-25 of about one each: 2^-11 both."""
+    n = 1 << 20
+    heads = 256                                   # (so many that one walk takes all keys)
+    q, k = torch.zeros(1, 1, 1, 64, dtype=F16, device="cuda"), torch.zeros(1, 1, n, 64, dtype=F16, device="cuda")
+    q[..., 0], k[:, :, 0, 0] = 4.0, 4.25
+    v = torch.ones(1, 1, n, 64, dtype=F16, device="cuda")
+    v[:, :, 0] = 0.0
+    k, v = k.expand(1, heads, n, 64), v.expand(1, heads, n, 64)
+    for rows in (1, 40):                          # one wave's rows, and a workgroup's
+        out, lse = lm.attention_forward(q.expand(1, heads, rows, 64), k, v, scale=1.0)
+        own = torch.arange(n - rows, n, device="cuda", dtype=torch.float64)[:, None]
+        total = own * torch.exp(torch.tensor(-17.0, dtype=torch.float64))
+        want = (total / (1 + total)).expand(rows, 64)
+        ref.within("out", out[0], want.expand(heads, rows, 64), 2.0 ** -10 * want)
+        assert float((lse[0].double() - (17 + torch.log1p(total[:, 0]))).abs().max()) <= 2.0 ** -11 + 2.0 ** -17 * 17
