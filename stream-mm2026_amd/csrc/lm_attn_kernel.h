@@ -620,12 +620,13 @@ __global__ __launch_bounds__(256, 6) void attn_delta_kernel(AttnArgs a)
     if (row < total && part == 0) a.delta[stat] = s;
 }
 
-// Scores that are hidden have no gradient, nor have those of LONE rows: their bits in `live` are 0.  Such rows
-// meet their key in tiles that are not all visible, the only ones to ask.
-__device__ __forceinline__ void settle(f32x16 &ds, uint32_t live)
+// Scores that are hidden have no gradient, nor have those of LONE rows: bit 16 + r of `bits` is 0 (bit r: whether
+// the score is visible; one word, for want of registers).  Such rows meet their key in tiles that are not all
+// visible, the only ones to ask.
+__device__ __forceinline__ void settle(f32x16 &ds, uint32_t bits)
 {
 #pragma unroll
-    for (int r = 0; r < 16; r++) ds[r] = (live >> r & 1) ? ds[r] : 0.0f;
+    for (int r = 0; r < 16; r++) ds[r] = (bits >> (16 + r) & 1) ? ds[r] : 0.0f;
 }
 
 // dq of WAVES x 32 rows: the forward pass's walk over the keys, 32 keys at a time so that scores, their
@@ -691,8 +692,11 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
         if (see != 0 && !sight.none(pa, pb, key, key + TILE - 1)) {
             const bool whole = see == ~0ull && sight.all(pa, pb, key, key + TILE - 1);
             for (int n = 0; n < 2; n++) {
-                uint32_t bits = 0;                           // which of the lane's 16 results are visible
-                if (!whole) bits = visible16(sight, pos, key + 32 * n, (uint32_t)(see >> (32 * n)), lane);
+                uint32_t bits = 0;                           // which of the lane's 16 results are visible; have a gradient
+                if (!whole) {
+                    bits = visible16(sight, pos, key + 32 * n, (uint32_t)(see >> (32 * n)), lane);
+                    bits |= is_lone(delta) ? 0 : bits << 16;
+                }
                 __builtin_amdgcn_sched_barrier(0);
                 f32x16 s = zero16(), dp = zero16();
     #pragma unroll
@@ -706,7 +710,7 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
                     s[r] = exp2_hw(__builtin_fmaf(s[r], c2, -lse));
                     dp[r] = s[r] * (dp[r] - delta);
                 }
-                if (!whole) settle(dp, is_lone(delta) ? 0 : bits);
+                if (!whole) settle(dp, bits);
                 lift.fit(dp, dq);
                 __builtin_amdgcn_sched_barrier(0);
     #pragma unroll
@@ -898,18 +902,17 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
         asm volatile("" : "+v"(rp), "+v"(cp));     // the reads' addresses are formed where they are used, not kept
         if (!sight.none(pa, pb, ka, ka + 31)) {
             const bool whole = all_seen && sight.all(pa, pb, ka, ka + 31);
-            uint32_t bits = 0, live = 0;                     // which of the lane's 16 results are visible; not LONE
+            uint32_t bits = 0;                               // which of the lane's 16 results are visible; have a gradient
             if (!whole) {
                 for (int r = 0; r < 16; r += 4) {
                     const u32x4 po = *(const u32x4 *)(pos_s[side] + result_row(r, lane));
                     const f32x4 de = *(const f32x4 *)(delta_s[side] + result_row(r, lane));
     #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        bits |= (uint32_t)(seen && sight.one((int)po[k], key)) << (r + k);
-                        live |= (uint32_t)!is_lone(de[k]) << (r + k);
+                        const bool one = seen && sight.one((int)po[k], key);
+                        bits |= ((uint32_t)one | (uint32_t)(one && !is_lone(de[k])) << 16) << (r + k);
                     }
                 }
-                live &= bits;
             }
             __builtin_amdgcn_sched_barrier(0);
             f32x16 s = zero16(), dp = zero16();
@@ -928,7 +931,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
                     dp[r + k] = s[r + k] * (dp[r + k] - de[k]);
                 }
             }
-            if (!whole) settle(dp, live);
+            if (!whole) settle(dp, bits);
             lift.fit(dp, dk);
             __builtin_amdgcn_sched_barrier(0);
     #pragma unroll
