@@ -25,6 +25,7 @@ extern "C" {
 /*
  * out[i, :] = scale * weight[tokens[i], :]; a token outside [0, vocab) gives a row of NaN.
  * weight: Float, BFloat16 or Half, rows weight_stride apart; out: [n, dim] dense, any of the three.
+ * n and vocab < 2^31, dim up to 2^24.
  */
 typedef struct stq_embedding {
     const void *tokens; /* [n], token_dtype STQ_LONG or STQ_INT */
@@ -42,7 +43,7 @@ int stq_embedding_forward(const stq_embedding *a, void *stream);
  * dweight[v, :] = scale * sum of grad[i, :] over tokens[i] == v, added in the order of i in fp32;
  * tokens outside [0, vocab) and `padding` (negative: none) add nothing.  accumulate: added to what
  * dweight holds (rows of no token are then left alone); otherwise every row is written.
- * n < 2^31, vocab < 2^31.  workspace: stq_embedding_grad_workspace(a) bytes, 16-byte aligned.
+ * n and vocab up to 2^30.  workspace: stq_embedding_grad_workspace(a) bytes, 16-byte aligned.
  */
 typedef struct stq_embedding_grad {
     const void *tokens;

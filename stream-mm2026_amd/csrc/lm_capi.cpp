@@ -70,6 +70,8 @@ int check_embedding_grad(const stq_embedding_grad *a)
 {
     if (!a) return bad("null arguments");
     CHECK(check_tokens(a->tokens, a->token_dtype, a->n, a->vocab, a->dim, a->scale));
+    CHECK(check_size("n", a->n, 0, lm::EMBED_GRAD_MAX));
+    CHECK(check_size("vocab", a->vocab, 1, lm::EMBED_GRAD_MAX));
     if (!is_float(a->grad_dtype)) return bad_type("grad", a->grad_dtype, FLOATS);
     if (!is_float(a->dweight_dtype)) return bad_type("dweight", a->dweight_dtype, FLOATS);
     return STQ_OK;

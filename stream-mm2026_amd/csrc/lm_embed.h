@@ -17,6 +17,9 @@ struct EmbedArgs {
 hipError_t embed_forward(const EmbedArgs &a, const void *weight, int weight_dt, int64_t weight_stride, void *out, int out_dt,
                          hipStream_t stream);
 
+// The gradient's kernels count tokens and rows in 32 bits and step past the last of them by up to a grid's surplus
+// (2^21 tokens, 512 rows), so that both stay below 2^31 up to here.
+constexpr int64_t EMBED_GRAD_MAX = 1 << 30;
 // Bytes of workspace that embed_backward needs.
 int64_t embed_backward_workspace(int64_t n, int64_t vocab, int64_t dim);
 
