@@ -65,7 +65,8 @@ int stq_embedding_backward(const stq_embedding_grad *a, void *stream);
  * n1 = norm(block; post_weight, post_bias), or block where post_weight is null
  * r  = residual_scale * x + gate * n1      (gate null: 1)
  * h  = norm(r; pre_weight, pre_bias)       r and h rounded once, h from the unrounded r
- * norm(y; w, c) = (y - mean) / sqrt(mean((y - mean)^2) + eps) * w + c; layer = 0: no mean is taken off.
+ * norm(y; w, c) = (y - mean) / sqrt(mean((y - mean)^2) + eps) * w + c; layer = 0: no mean is taken off,
+ * and there are no biases.
  * Rows of `dim` elements, 8 <= dim <= 8192; x, block, dr, dh strided, the others dense.  gate:
  * [groups, dim], row i takes gate[i / (n / groups)], groups divides n.  weight_dtype: Float or dtype.
  * stats: [n, 4] floats that the forward call writes and the backward call reads.

@@ -89,6 +89,7 @@ int check_norm(const stq_norm_residual *a, bool backward)
     if (!std::isfinite(a->residual_scale)) return bad("residual_scale must be finite");
     if (!a->pre_weight) return bad("pre_weight: null data pointer");
     if (a->post_bias && !a->post_weight) return bad("post_bias needs post_weight");
+    if (!a->layer && (a->pre_bias || a->post_bias)) return bad("biases need layer norms (layer = 1)");
     if (a->gate) {
         CHECK(check_size("gate rows", a->groups, 1, a->n > 0 ? a->n : 1));
         if (a->n % a->groups)

@@ -4,7 +4,7 @@ import pytest
 
 import stquant_lm as lm
 from mdq_hip import _capi
-from test_lm_cpu import INVALID, embed_grad, err
+from test_lm_cpu import INVALID, embed_grad, err, norm
 
 
 def embed_grad_workspace(**kw):
@@ -36,3 +36,11 @@ def last_index(n, threads=64, seg=16):
 def test_the_limit_is_what_the_grid_needs():
     assert last_index(1 << 30) < 1 << 31
     assert last_index((1 << 31) - 1) >= 1 << 31          # (what was accepted before)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("kw", [dict(pb=0x10000, dpb=0x10000), dict(qw=0x10000, qb=0x10000, dqw=0x10000, dqb=0x10000)])
+def test_rms_norms_refuse_biases(backward, kw):
+    """They were accepted and left out of the result."""
+    kw = kw if backward else {k: v for k, v in kw.items() if k[0] != "d"}
+    assert norm(backward, **kw) == INVALID and "biases need layer norms" in err()
