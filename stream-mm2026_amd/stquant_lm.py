@@ -7,8 +7,9 @@ What a training step runs around the optimizer, each with its gradient:
 ``attention``      causal attention over a window of the last keys and a few first ones (sinks)
 ``distill_loss``   learning from a teacher's top logits, mixed with the labels' cross-entropy
 
-The plain names are differentiable (``torch.autograd``); the ``*_forward`` / ``*_backward`` pairs and
-``distill_loss_and_grad`` are the calls beneath them, for training loops that hold their own buffers.
+The plain names are differentiable (``torch.autograd``), once: a second derivative raises.  The
+``*_forward`` / ``*_backward`` pairs and ``distill_loss_and_grad`` are the calls beneath them, for
+training loops that hold their own buffers.
 Everything runs on the current stream of the tensors' device through the C ABI of
 ``include/stquant_lm.h``; nothing synchronises, so calls can be captured into a graph.  As with torch's
 own operators, a tensor used on another stream than the one it was allocated on is the caller's to keep
@@ -23,6 +24,7 @@ import sys
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 if _HERE not in sys.path:
@@ -166,6 +168,7 @@ class _Embedding(torch.autograd.Function):
         return embedding_forward(tokens, weight, scale=scale, dtype=dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         (tokens,) = ctx.saved_tensors
         n, scale, padding_idx, dtype = ctx.args
@@ -272,6 +275,7 @@ class _NormResidual(torch.autograd.Function):
         return r, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dr, dh):
         x, block, pre_weight, pre_bias, post_weight, post_bias, gate, stats = ctx.saved_tensors
         if dh is None:
@@ -399,6 +403,7 @@ class _Attention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, key_mask = ctx.saved_tensors
         return (*attention_backward(dout, q, k, v, out, lse, key_mask=key_mask, **ctx.args), None, None, None, None)
@@ -508,6 +513,7 @@ class _DistillLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         logits, teacher_logits, teacher_ids, labels, stats = ctx.saved_tensors
         dz = distill_loss_backward(grad, logits, teacher_logits, teacher_ids, stats, labels=labels, **ctx.args)
