@@ -99,6 +99,14 @@ def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     return t if t.stride(1) == 1 or width == 1 else t.contiguous()
 
 
+def _written(*tensors: torch.Tensor) -> None:
+    """Tensors of the caller that a call has written count as changed in place: autograd then refuses to use one that
+    another operation saved."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _workspace(nbytes: int, dev: torch.device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
@@ -157,6 +165,8 @@ def embedding_backward(grad: torch.Tensor, tokens: torch.Tensor, num_embeddings:
     ws = _workspace(_size(L.stq_embedding_grad_workspace, _EMBED_GRAD.pack(*args)), grad.device)
     args[13:15] = ws.data_ptr(), ws.numel()
     _call(grad.device, L.stq_embedding_backward, _EMBED_GRAD.pack(*args))
+    if out is not None:
+        _written(out)
     return dw
 
 
@@ -376,7 +386,8 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
         _fail(f"lse must be the forward call's [{b}, {h}, {t}]")
     _same_device(q, dout=dout, out=out, lse=lse)
     q, k, v, out, dout = map(_piecewise, (q, k, v, out, dout))
-    if grads is None:
+    given = grads is not None
+    if not given:
         grads = tuple(torch.empty((b, n, heads, d), dtype=q.dtype, device=q.device).transpose(1, 2) for n, heads in ((t, h), (s, hk), (s, hk)))
     else:
         for name, x, like in zip(("dq", "dk", "dv"), grads, (q, k, v)):
@@ -391,6 +402,8 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     if ws is not None:
         args[-2:] = ws.data_ptr(), ws.numel()
     _call(q.device, L.stq_attention_backward, _ATTN.pack(*args))
+    if given:
+        _written(dq, dk, dv)
     return dq, dk, dv
 
 
@@ -483,11 +496,13 @@ def distill_loss_backward(grad, logits: torch.Tensor, teacher_logits: torch.Tens
     if stats.dtype != torch.float32 or stats.shape != (z.shape[0], 4) or not stats.is_contiguous():
         _fail(f"stats must be the forward call's [{z.shape[0]}, 4]")
     w = _row_weights(grad, z, logits.shape[:-1])
-    out, rows = _grad_rows(logits, z, out)
+    dz, rows = _grad_rows(logits, z, out)
     _same_device(z, stats=stats)
     _call(z.device, lm_lib().stq_distill_backward,
           _DISTILL.pack(*head, 0, stats.data_ptr(), w.data_ptr(), rows.data_ptr(), rows.stride(0)))
-    return out
+    if out is not None:
+        _written(out)
+    return dz
 
 
 def distill_loss_and_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, *, grad,
@@ -498,10 +513,12 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, te
     z, keep, head = _distill(logits, teacher_logits, teacher_ids, labels, temperature, alpha)
     w = _row_weights(grad, z, logits.shape[:-1])
     loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=z.device)
-    out, rows = _grad_rows(logits, z, out)
+    dz, rows = _grad_rows(logits, z, out)
     _call(z.device, lm_lib().stq_distill_forward,
           _DISTILL.pack(*head, loss.data_ptr(), 0, w.data_ptr(), rows.data_ptr(), rows.stride(0)))
-    return loss, out
+    if out is not None:
+        _written(out)
+    return loss, dz
 
 
 class _DistillLoss(torch.autograd.Function):
