@@ -541,6 +541,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a)
 // weights, which lse's rounding leaves off 1: a weight of 1 - 2^-17 beside one of 2^-17 keeps its gradient.  A row
 // that sees one key has no score gradient at all: its delta says LONE.
 constexpr int FEW_KEYS = 16;
+constexpr int DELTA_Y = 32768;                     // 16 rows each along the grid's second dimension, the rest along the third
 constexpr uint32_t LONE = 0x7fc01e01u;             // a NaN of these bits
 __device__ __forceinline__ bool is_lone(float delta) { return __builtin_bit_cast(uint32_t, delta) == LONE; }
 
@@ -550,8 +551,9 @@ __global__ __launch_bounds__(256, 6) void attn_delta_kernel(AttnArgs a)
     __shared__ int list_[16][FEW_KEYS];
     const int lane = threadIdx.x & 63, part = lane & 15;
     // (the first rows of all heads first: they see the fewest keys and take longest)
-    const int heads = a.batch * a.key_heads, y = blockIdx.x % heads, b = y / a.key_heads, hk = y % a.key_heads;
-    const int total = a.rows * a.group, row = blockIdx.x / heads * 16 + (threadIdx.x >> 4), rr = min(row, total - 1);
+    const int b = blockIdx.x / a.key_heads, hk = blockIdx.x % a.key_heads;
+    const int total = a.rows * a.group, row = (blockIdx.z * DELTA_Y + blockIdx.y) * 16 + (threadIdx.x >> 4), rr = min(row, total - 1);
+    if (row - (int)(threadIdx.x >> 4) >= total) return;
     const int t = rr / a.group, h = hk * a.group + rr % a.group, pos = a.keys - a.rows + t;
     const int64_t stat = ((int64_t)b * a.heads + h) * a.rows + t;
     const uint16_t *o = at(a.o, b, h) + t * a.o.t, *g = at(a.dout, b, h) + t * a.dout.t;
@@ -1016,28 +1018,42 @@ __global__ __launch_bounds__(256) void attn_parts_kernel(AttnArgs a, DkvSplit cu
     *(uint32_t *)((uint16_t *)at(a.dv, b, hk) + (int64_t)key * a.dv.t + e) = pack2<DT>(v[0], v[1]);
 }
 
+// (A launch's error is read before the next one: that one's success would take its place.)
 template <int DT, int HD>
-void run_forward(const AttnArgs &a, hipStream_t stream)
+hipError_t run_forward(const AttnArgs &a, hipStream_t stream)
 {
     const int total = a.rows * a.group, heads = a.batch * a.key_heads;
     if (total <= 32)
         attn_fwd_kernel<DT, HD, 1><<<dim3(heads, 1, a.splits), 64, 0, stream>>>(a);
     else
         attn_fwd_kernel<DT, HD, 4><<<dim3(heads, (total + 127) / 128, a.splits), 256, 0, stream>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.splits == 1) return e;
     if (a.splits > FEW) attn_join_kernel<DT><<<dim3(heads, total), 256, 0, stream>>>(a);
-    else if (a.splits > 1) attn_join_few_kernel<DT><<<dim3(heads, (total + 3) / 4), 256, 0, stream>>>(a);
+    else attn_join_few_kernel<DT><<<dim3(heads, (total + 3) / 4), 256, 0, stream>>>(a);
+    return hipGetLastError();
 }
 
 template <int DT, int HD>
-void run_backward(const AttnArgs &a, hipStream_t stream)
+hipError_t run_backward(const AttnArgs &a, hipStream_t stream)
 {
     const int total = a.rows * a.group, heads = a.batch * a.key_heads;
     const int64_t rows = (int64_t)a.batch * a.heads * a.rows;
     const DkvSplit cut = dkv_split(a);
-    if (rows) attn_delta_kernel<DT><<<(unsigned)((total + 15) / 16) * heads, 256, 0, stream>>>(a);
+    hipError_t e = hipSuccess;
+    if (rows) {
+        const int tiles = (total + 15) / 16;
+        attn_delta_kernel<DT><<<dim3(heads, tiles < DELTA_Y ? tiles : DELTA_Y, (tiles + DELTA_Y - 1) / DELTA_Y), 256, 0, stream>>>(a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     attn_dkv_kernel<DT, HD, 4><<<dim3(heads, cut.blocks * cut.shares + cut.sink_blocks * cut.far), 256, 0, stream>>>(a, cut);
-    if (cut.parts() > 1) attn_parts_kernel<DT><<<dim3(heads, (unsigned)(((int64_t)cut.keys(a) * a.dim / 2 + 255) / 256)), 256, 0, stream>>>(a, cut);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (cut.parts() > 1) {
+        attn_parts_kernel<DT><<<dim3(heads, (unsigned)(((int64_t)cut.keys(a) * a.dim / 2 + 255) / 256)), 256, 0, stream>>>(a, cut);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     if (rows) attn_dq_kernel<DT, HD, 4><<<dim3(heads, (total + 127) / 128), 256, 0, stream>>>(a);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -1045,17 +1061,13 @@ void run_backward(const AttnArgs &a, hipStream_t stream)
 template <int DT>
 hipError_t attn_forward(const AttnArgs &a, hipStream_t stream)
 {
-    if (a.dim <= 64) run_forward<DT, 64>(a, stream);
-    else run_forward<DT, 128>(a, stream);
-    return hipGetLastError();
+    return a.dim <= 64 ? run_forward<DT, 64>(a, stream) : run_forward<DT, 128>(a, stream);
 }
 
 template <int DT>
 hipError_t attn_backward(const AttnArgs &a, hipStream_t stream)
 {
-    if (a.dim <= 64) run_backward<DT, 64>(a, stream);
-    else run_backward<DT, 128>(a, stream);
-    return hipGetLastError();
+    return a.dim <= 64 ? run_backward<DT, 64>(a, stream) : run_backward<DT, 128>(a, stream);
 }
 
 }  // namespace lm

@@ -21,3 +21,16 @@ def test_distillation_of_more_rows_than_a_launch_dimension():
     want = torch.full((n, v), 0.125, dtype=torch.bfloat16, device="cuda")
     want.scatter_(1, ids.long(), -0.875)
     assert torch.equal(dz, want) and torch.equal(two, want)
+
+
+def test_attention_gradients_of_more_rows_than_a_launch_dimension():
+    """A window of one key: out is v, dv is dout and the scores have no gradients, all exactly."""
+    b, h, t, d = 1, 65535, 4099, 8
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randint(-8, 9, (b, h, t, d), dtype=torch.int8, device="cuda", generator=g).to(torch.bfloat16)
+    do = x + 1
+    out, lse = lm.attention_forward(x, x, x, window=1)
+    assert torch.equal(out, x)
+    dq, dk, dv = lm.attention_backward(do, x, x, x, out, lse, window=1)
+    assert torch.equal(dv, do)
+    assert not bool(dq.any()) and not bool(dk.any())
