@@ -26,6 +26,7 @@ namespace {
 constexpr int SEG = 16;            // sorted entries per wave of the sums
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
 constexpr int MAX_RANGE = 512;     // rows of the vocabulary that one workgroup sorts (its LDS counters)
+constexpr int LOOKUP_X = 1 << 22;  // workgroups of the lookup along a grid's first dimension, which ends at 2^32 threads
 constexpr int LIST = 256;          // entries a wave of the sort keeps in LDS before it reads them again
 
 __device__ __forceinline__ int64_t token_at(const void *tokens, int bytes, int64_t i)
@@ -42,7 +43,8 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void *tokens, int 
                                                         float scale, const void *weight, int64_t weight_stride, void *out,
                                                         int rows_per_wg, int pieces)
 {
-    const int64_t row0 = (int64_t)blockIdx.x * rows_per_wg;
+    const int64_t row0 = ((int64_t)blockIdx.z * LOOKUP_X + blockIdx.x) * rows_per_wg;
+    if (row0 >= n) return;
     const int rows = (int)min((int64_t)rows_per_wg, n - row0);
     const int total = rows * pieces;
     for (int c0 = blockIdx.y * 1024 + threadIdx.x; c0 < total; c0 += gridDim.y * 1024) {
@@ -331,7 +333,9 @@ void launch_fwd(const EmbedArgs &a, const void *weight, int64_t weight_stride, v
     const bool wide = aligned(weight, weight_stride, a.dim, 8, size_of(WDT)) && aligned(out, a.dim, a.dim, 8, size_of(ODT));
     const int pieces = (int)(wide ? a.dim / 8 : a.dim);
     const int rows = pieces >= 1024 ? 1 : 1024 / pieces;
-    const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)((rows * pieces + 1023) / 1024));
+    const int64_t wgs = (a.n + rows - 1) / rows;
+    const dim3 grid((unsigned)(wgs < LOOKUP_X ? wgs : LOOKUP_X), (unsigned)((rows * pieces + 1023) / 1024),
+                    (unsigned)((wgs + LOOKUP_X - 1) / LOOKUP_X));
     if (wide)
         embed_fwd_kernel<WDT, ODT, 8><<<grid, 256, 0, stream>>>(a.tokens, a.token_bytes, a.n, a.vocab, (int)a.dim, a.scale, weight,
                                                                 weight_stride, out, rows, pieces);
@@ -341,7 +345,7 @@ void launch_fwd(const EmbedArgs &a, const void *weight, int64_t weight_stride, v
 }
 
 template <int GDT, int DWDT, int VEC>
-void launch_bwd(const EmbedArgs &a, const void *grad, int64_t grad_stride, void *dweight, int64_t dweight_stride, int64_t padding,
+hipError_t launch_bwd(const EmbedArgs &a, const void *grad, int64_t grad_stride, void *dweight, int64_t dweight_stride, int64_t padding,
                 bool accumulate, void *workspace, hipStream_t stream)
 {
     int *tok = (int *)workspace;
@@ -354,28 +358,30 @@ void launch_bwd(const EmbedArgs &a, const void *grad, int64_t grad_stride, void 
     embed_sort_kernel<DWDT, VEC><<<(unsigned)((a.vocab + range - 1) / range), SORT_THREADS, 0, stream>>>(
         a.tokens, a.token_bytes, (int)a.n, (int)a.vocab, range, bits, padding, tok, pos, count, dweight, dweight_stride, (int)a.dim,
         !accumulate);
-    if (a.n == 0) return;
+    // (an error is read before the next launch, whose success would take its place)
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.n == 0) return e;
     const int64_t pieces = a.dim / VEC;
     // (the slices of a chunk's columns side by side: their rows' lines are neighbours in memory)
     const int64_t wgs = (chunks(a.n) + 3) / 4;
     const dim3 grid((unsigned)((pieces + 63) / 64), (unsigned)(wgs < 32768 ? wgs : 32768), (unsigned)((wgs + 32767) / 32768));
     embed_sum_kernel<GDT, DWDT, VEC><<<grid, 256, 0, stream>>>(tok, pos, count, grad, grad_stride, (int)a.dim, a.scale, dweight,
                                                                dweight_stride, accumulate, partial);
-    if (a.n > SEG)
-        embed_join_kernel<DWDT, VEC><<<grid, 256, 0, stream>>>(tok, count, (int)a.dim, a.scale, dweight, dweight_stride, accumulate,
-                                                               partial);
+    e = hipGetLastError();
+    if (e != hipSuccess || a.n <= SEG) return e;
+    embed_join_kernel<DWDT, VEC><<<grid, 256, 0, stream>>>(tok, count, (int)a.dim, a.scale, dweight, dweight_stride, accumulate, partial);
+    return hipGetLastError();
 }
 
 template <int GDT, int DWDT>
-void pick_bwd(const EmbedArgs &a, const void *grad, int64_t gs, void *dw, int64_t dws, int64_t padding, bool acc, void *ws,
+hipError_t pick_bwd(const EmbedArgs &a, const void *grad, int64_t gs, void *dw, int64_t dws, int64_t padding, bool acc, void *ws,
               hipStream_t stream)
 {
     // 4 columns a lane where a row of fp32 is involved (16 bytes of it), 8 where all are 16-bit
     constexpr int WIDE = GDT == DT_F32 || DWDT == DT_F32 ? 4 : 8;
     if (aligned(grad, gs, a.dim, WIDE, size_of(GDT)) && aligned(dw, dws, a.dim, WIDE, size_of(DWDT)))
-        launch_bwd<GDT, DWDT, WIDE>(a, grad, gs, dw, dws, padding, acc, ws, stream);
-    else
-        launch_bwd<GDT, DWDT, 1>(a, grad, gs, dw, dws, padding, acc, ws, stream);
+        return launch_bwd<GDT, DWDT, WIDE>(a, grad, gs, dw, dws, padding, acc, ws, stream);
+    return launch_bwd<GDT, DWDT, 1>(a, grad, gs, dw, dws, padding, acc, ws, stream);
 }
 
 }  // namespace
@@ -411,10 +417,11 @@ int64_t embed_backward_workspace(int64_t n, int64_t vocab, int64_t dim)
 hipError_t embed_backward(const EmbedArgs &a, const void *grad, int grad_dt, int64_t grad_stride, void *dweight, int dweight_dt,
                           int64_t dweight_stride, int64_t padding, bool accumulate, void *workspace, hipStream_t stream)
 {
-#define CALL(G, W) pick_bwd<G, W>(a, grad, grad_stride, dweight, dweight_stride, padding, accumulate, workspace, stream)
+    hipError_t e = hipSuccess;
+#define CALL(G, W) e = pick_bwd<G, W>(a, grad, grad_stride, dweight, dweight_stride, padding, accumulate, workspace, stream)
     LM_TYPE_PAIR(grad_dt, dweight_dt, CALL)
 #undef CALL
-    return hipGetLastError();
+    return e;
 }
 
 }  // namespace lm

@@ -34,3 +34,14 @@ def test_attention_gradients_of_more_rows_than_a_launch_dimension():
     dq, dk, dv = lm.attention_backward(do, x, x, x, out, lse, window=1)
     assert torch.equal(dv, do)
     assert not bool(dq.any()) and not bool(dk.any())
+
+
+def test_lookup_of_more_rows_than_a_launch_dimension():
+    n, vocab, dim = (1 << 24) + 77, 5, 515
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.randn(vocab, dim, device="cuda", generator=g).to(torch.bfloat16)
+    tok = torch.arange(n, device="cuda", dtype=torch.int32) % vocab
+    out = lm.embedding_forward(tok, w)
+    for a in range(0, n, 1 << 21):
+        b = min(n, a + (1 << 21))
+        assert torch.equal(out[a:b], w[tok[a:b].long()]), a
