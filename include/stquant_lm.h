@@ -68,7 +68,8 @@ int stq_embedding_backward(const stq_embedding_grad *a, void *stream);
  * norm(y; w, c) = (y - mean) / sqrt(mean((y - mean)^2) + eps) * w + c; layer = 0: no mean is taken off,
  * and there are no biases.
  * Rows of `dim` elements, 8 <= dim <= 8192; x, block, dr, dh strided, the others dense.  gate:
- * [groups, dim], row i takes gate[i / (n / groups)], groups divides n.  weight_dtype: Float or dtype.
+ * [groups, dim], row i takes gate[i / (n / groups)], groups divides n (0: up to 2^30 of them).
+ * weight_dtype: Float or dtype.
  * stats: [n, 4] floats that the forward call writes and the backward call reads.
  */
 typedef struct stq_norm_residual {

@@ -91,7 +91,7 @@ int check_norm(const stq_norm_residual *a, bool backward)
     if (a->post_bias && !a->post_weight) return bad("post_bias needs post_weight");
     if (!a->layer && (a->pre_bias || a->post_bias)) return bad("biases need layer norms (layer = 1)");
     if (a->gate) {
-        CHECK(check_size("gate rows", a->groups, 1, a->n > 0 ? a->n : 1));
+        CHECK(check_size("gate rows", a->groups, 1, a->n > 0 ? a->n : 1 << 30));
         if (a->n % a->groups)
             return fail(STQ_ERR_INVALID, "gate rows (%lld) must divide the rows (%lld)", (long long)a->groups, (long long)a->n);
     }

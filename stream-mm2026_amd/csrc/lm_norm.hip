@@ -11,19 +11,22 @@ namespace {
 int most_wgs(int waves) { return waves <= 4 ? 1024 : waves <= 8 ? 512 : 256; }
 
 // Adds the partial rows: blockIdx.y names the sum (4 and up: the groups of the gate).  64 columns a
-// workgroup, its 16 waves take every 16th partial row.  1024 partial rows of 768 4.5 us, 512 of 4096 9.4 us.
+// workgroup, its 16 waves take every 16th partial row (without rows there are none: zeros, for any number of
+// groups, those beyond GATES_Y along blockIdx.z).  1024 partial rows of 768 4.5 us, 512 of 4096 9.4 us.
+constexpr int GATES_Y = 32768;
 __global__ __launch_bounds__(1024) void norm_finish_kernel(NormArgs a, NormSplit sp)
 {
     __shared__ float buf[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int which = min((int)blockIdx.y, 4);
     void *out = which == 0 ? a.dpre_weight : which == 1 ? a.dpre_bias : which == 2 ? a.dpost_weight : which == 3 ? a.dpost_bias : a.dgate;
-    if (!out) return;
+    const int64_t group = (int64_t)blockIdx.z * GATES_Y + blockIdx.y - 4;
+    if (!out || (which == 4 ? group >= a.groups : blockIdx.z != 0)) return;
     int64_t first = 0, rows = sp.wgs, to = 0;
     if (which == 4) {
-        first = (int64_t)(blockIdx.y - 4) * sp.per_group;
+        first = group * sp.per_group;
         rows = sp.per_group;
-        to = (int64_t)(blockIdx.y - 4) * a.dim;
+        to = group * a.dim;
     }
     const int64_t col = (int64_t)blockIdx.x * 64 + lane;
     float s = 0.0f;
@@ -90,8 +93,9 @@ hipError_t by_type(const NormArgs &a, bool backward, hipStream_t stream)
             : a.weight_dt                    ? norm_run<DT_F16, false>(a, sp, ragged, backward, stream)
                                              : norm_run<DT_F16, true>(a, sp, ragged, backward, stream);
     if (e != hipSuccess || !backward) return e;
-    const unsigned sums = a.gate && (sp.per_group || !a.n) ? 4 + (unsigned)a.groups : 4;
-    norm_finish_kernel<<<dim3((unsigned)((a.dim + 63) / 64), sums), 1024, 0, stream>>>(a, sp);
+    const int64_t gates = a.gate && (sp.per_group || !a.n) ? a.groups : 0;
+    norm_finish_kernel<<<dim3((unsigned)((a.dim + 63) / 64), 4 + (unsigned)(gates < GATES_Y ? gates : GATES_Y),
+                              gates ? (unsigned)((gates + GATES_Y - 1) / GATES_Y) : 1), 1024, 0, stream>>>(a, sp);
     return hipGetLastError();
 }
 

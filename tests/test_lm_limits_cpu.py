@@ -44,3 +44,11 @@ def test_rms_norms_refuse_biases(backward, kw):
     """They were accepted and left out of the result."""
     kw = kw if backward else {k: v for k, v in kw.items() if k[0] != "d"}
     assert norm(backward, **kw) == INVALID and "biases need layer norms" in err()
+
+
+def test_a_gate_of_several_groups_without_rows():
+    """No rows divide into any number of groups; what cannot be (rows and no group, a grid of sums beyond 65535) is refused."""
+    assert norm(False, n=0, gate=0x10000, groups=5, x=0, block=0, r=0, h=0, stats=0) == _capi.STQ_OK
+    for kw, msg in [(dict(gate=0x10000, groups=0), "gate rows must be 1 to 4"), (dict(n=0, gate=0x10000, groups=0), "gate rows must be 1 to"),
+                    (dict(n=0, gate=0x10000, groups=1 << 31), "gate rows must be 1 to")]:
+        assert norm(False, **kw) == INVALID and msg in err()
