@@ -116,3 +116,22 @@ def test_nothing_behind_a_row_is_written(n, v, dtype):
     _, stats = lm.distill_loss_forward(z[:, :v], t, ids)
     lm.distill_loss_backward(1.0, z[:, :v], t, ids, stats, out=out[:, :v])
     assert bool((out[:, v:] == 7).all())
+
+
+@pytest.mark.parametrize("v", [1000, 12000, 50257, 60000])
+@pytest.mark.parametrize("temp,top", [(1e-9, 11.0), (1e-4, 11.0), (2.0, 3e38), (3.0, -3e38), (4.0, 1e9)])
+def test_many_rows_of_steep_logits(v, temp, top):
+    """The instances for more than 512 rows, in place: rows of a value and of ones far below it."""
+    n, k = 520, 3
+    z = torch.full((n, v), top, device="cuda").to(BF16)
+    z[:, 5:] = -z[:, 5:].abs() / 2 if top > 0 else float("-inf")
+    ids = torch.arange(k, device="cuda").expand(n, k).contiguous()
+    t = torch.zeros(n, k, dtype=BF16, device="cuda")
+    w = torch.full((n,), 1.0, device="cuda")
+    loss, dz = lm.distill_loss_and_grad(z, t, ids, grad=w, temperature=temp, out=z)
+    # uniform over 5, the teacher over 3 of them
+    want = torch.zeros(n, v, dtype=torch.float64, device="cuda")
+    want[:, :5] = temp / 5
+    want[:, :3] -= temp / 3
+    ref.within("loss", loss, torch.full((n,), temp * temp * 0.5108256237659907, dtype=torch.float64, device="cuda"), 2.0 ** -16 * temp * temp)
+    ref.within("dlogits", dz, want, 2.0 ** -16 * temp * (want != 0))

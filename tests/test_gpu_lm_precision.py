@@ -149,3 +149,32 @@ def test_fp16_a_key_far_above_many():
         want = (total / (1 + total)).expand(rows, 64)
         ref.within("out", out[0], want.expand(heads, rows, 64), 2.0 ** -10 * want)
         assert float((lse[0].double() - (17 + torch.log1p(total[:, 0]))).abs().max()) <= 2.0 ** -11 + 2.0 ** -17 * 17
+
+
+@pytest.mark.parametrize("d,group,window,sinks", [(64, 1, 64, 3), (128, 1, 100, 200), (64, 3, 1, 1), (128, 2, 300, 128)])
+def test_every_far_row_reaches_the_sinks(d, group, window, sinks):
+    """dout is zero in all rows of a head but one: what the sinks' keys get is that row's, wherever the walk is cut.
+
+    Rows around every multiple of 32 behind the window, one a head, so that a row lost at any border leaves dv zero."""
+    t, hk = 1600, 40
+    h = hk * group
+    rows = [p + i for p in range(window + sinks + 130, t, 64) for i in (-1, 0, 1)][: 4 * h]
+    g = ref.gen(window)
+    q = ref.randn(g, 4, h, t, d, std=0.3, dtype=F16)
+    k, v = (ref.randn(g, 4, hk, t, d, std=0.3, dtype=F16) for _ in range(2))
+    do = torch.zeros_like(q)
+    at = [(i // h, i % h, p) for i, p in enumerate(rows)]
+    for b, j, p in at:
+        do[b, j, p] = ref.randn(g, d, std=30.0, dtype=F16)
+    out, lse = lm.attention_forward(q, k, v, window=window, sinks=sinks)
+    dv = lm.attention_backward(do, q, k, v, out, lse, window=window, sinks=sinks)[2]
+    want = torch.zeros(4, hk, t, d, dtype=torch.float64, device="cuda")
+    mag = torch.zeros_like(want)
+    see = ref.visible(t, t, window, sinks, None, 1, "cuda")[0]
+    for b, j, p in at:
+        s = (q[b, j, p].double() @ k[b, j // group].double().t().contiguous() * d ** -0.5).masked_fill(~see[p], ref.NEG)
+        w = torch.softmax(s, -1)[:, None] * do[b, j, p].double()[None]
+        want[b, j // group] += w
+        mag[b, j // group] += w.abs()
+    assert float(want[:, :, :sinks].abs().amax()) > 0.01
+    ref.within("dv", dv, want, (ref.U[F16] + ref.F32) * mag)
