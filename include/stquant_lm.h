@@ -109,6 +109,7 @@ typedef struct stq_tensor4 {
  * 2^22, head_stride >= 0 and of q and dout, times heads / key_heads, up to 2^29.
  * out is rounded once; softmax weights and the gradients of the scores are rounded to dtype before the
  * products with them (those of Half times a power of two that keeps them among its normal numbers).
+ * A weight carries fp32's error of its score and of lse, 2^-24 of their size: scores should stay below 2^24.
  * lse: [batch, heads, rows] floats, written forward, read backward.
  */
 typedef struct stq_attention {

@@ -98,7 +98,10 @@ struct Tile {
     }
 };
 
-// 8 results (registers r0 .. r0 + 7) rounded to the B operand of 16 k.
+// 8 results (registers r0 .. r0 + 7) rounded to the B operand of 16 k: the matrix instructions take 16 bits.  Weights
+// and score gradients as two parts each in every tile would make the outputs those of products in fp32 (errors 1.00
+// to 1.02 times theirs; so 1.22 to 1.40) and took 161 us in place of 141 (8 x 12 x 1024 of 64, with gradients), 1805 in
+// place of 1332 (8192 positions of 32 heads of 128, window 2048) and 157 in place of 122 (fp16, ragged).
 template <int DT>
 __device__ __forceinline__ u32x4 operand(const f32x16 &s, int r0)
 {
@@ -114,8 +117,8 @@ constexpr float RAISE = DT == DT_F16 ? 14.0f : 0.0f;
 
 // What that rounding left, as an operand of its own.  Rows that see few keys have the largest score
 // gradients, and the tiles in which they see them are not all visible: only there dS is multiplied as
-// two parts (dq of 8 x 12 x 1024 of 64: 1.49 times the error of a product in fp32 before, 1.35 now, for
-// 2 us of 37).
+// two parts (dq of 8 x 12 x 1024 of 64: 1.49 times the error of a product in fp32 before, 1.35 with it for
+// 2 us of 37, and 1.27 with delta as below).
 template <int DT>
 __device__ __forceinline__ u32x4 remainder(const f32x16 &s, int r0, u32x4 rounded)
 {
@@ -312,8 +315,8 @@ __device__ __forceinline__ const uint16_t *at(const AttnTensor &t, int b, int h)
 // issue: per score two products of the head size against one exponential and about six vector instructions,
 // so most of a tile's cycles are the softmax's.  A maximum that does not grow skips the rescaling.  Tiles of
 // up to 32 rows run as one wave, where latency counts.  Window 2048 with 4 sinks over 8192 positions, 32
-// heads of 128 on 8 of keys, bf16: 305-333 us, 0.8 PFLOP/s of visible products; 12 heads of 64, 8 x 1024
-// causal: 31 us.
+// heads of 128 on 8 of keys, bf16: 300-310 us, 0.8 PFLOP/s of visible products; 12 heads of 64, 8 x 1024
+// causal: 30 us.
 template <int DT, int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void attn_fwd_kernel(AttnArgs a)
 {
@@ -366,21 +369,21 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
         asm volatile("" : "+v"(rp), "+v"(cp));     // the reads' addresses are formed where they are used, not kept
         if (see != 0 && !sight.none(pa, pb, key, key + TILE - 1)) {
             f32x16 s[2] = {zero16(), zero16()};
-    #pragma unroll
+#pragma unroll
             for (int c = 0; c < C; c++)
-    #pragma unroll
+#pragma unroll
                 for (int n = 0; n < 2; n++) s[n] = mma<DT>(Tile<HD>::rows(kt, rp, 32 * n, c), q[c], s[n]);
             if (see != ~0ull || !sight.all(pa, pb, key, key + TILE - 1)) {
-    #pragma unroll
+#pragma unroll
                 for (int n = 0; n < 2; n++) {
                     const uint32_t bits = visible16(sight, pos, key + 32 * n, (uint32_t)(see >> (32 * n)), lane);
                     hide(s[n], bits);
                 }
             }
             float top = s[0][0];
-    #pragma unroll
+#pragma unroll
             for (int n = 0; n < 2; n++)
-    #pragma unroll
+#pragma unroll
                 for (int r = 0; r < 16; r++) top = fmaxf(top, s[n][r]);
             top = both_halves(top, [](float x, float y) { return fmaxf(x, y); }) * c2;
             if (__ballot(top > m)) {
@@ -388,27 +391,27 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 1 ? 1 : HD == 64 ? 3 : 2) void
                 const float keep = m == now ? 1.0f : exp2_hw(m - now);     // (both -inf: nothing yet)
                 m = now;
                 l *= keep;
-    #pragma unroll
+#pragma unroll
                 for (int d = 0; d < ND; d++)
-    #pragma unroll
+#pragma unroll
                     for (int r = 0; r < 16; r++) o[d][r] *= keep;
             }
             const float ref = (m == -__builtin_inff() ? 0.0f : m) - RAISE<DT>;
             float sum = 0.0f;              // (added to l once a tile: beside a large l single weights would be lost)
-    #pragma unroll
+#pragma unroll
             for (int n = 0; n < 2; n++)
-    #pragma unroll
+#pragma unroll
                 for (int r = 0; r < 16; r++) {
                     s[n][r] = exp2_hw(__builtin_fmaf(s[n][r], c2, -ref));
                     sum += s[n][r];
                 }
             l += sum;
-    #pragma unroll
+#pragma unroll
             for (int n = 0; n < 2; n++)
-    #pragma unroll
+#pragma unroll
                 for (int k = 0; k < 2; k++) {
                     const u32x4 p = operand<DT>(s[n], 8 * k);
-    #pragma unroll
+#pragma unroll
                     for (int d = 0; d < ND; d++) o[d] = mma<DT>(Tile<HD>::columns(vt, cp, 32 * n + 16 * k, d), p, o[d]);
                 }
         }
@@ -537,7 +540,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a)
 // delta = rowsum(dout * out): 16 lanes a row.  A row that sees up to FEW_KEYS keys takes sum P (do v^T) from
 // them instead: `out` is rounded, and what that puts into delta falls with the number of keys, while the
 // rounding of dS does not (a handful of positions: the error of dq 1.05 times that of products in fp32, 2.3
-// before; 8 x 12 x 1024 of 64 11 us, 6 before; a wave a row in turn 38).  It is divided by the sum of the same
+// before; 8 x 12 x 1024 of 64 10 us, 6 before; a wave a row in turn 38).  It is divided by the sum of the same
 // weights, which lse's rounding leaves off 1: a weight of 1 - 2^-17 beside one of 2^-17 keeps its gradient.  A row
 // that sees one key has no score gradient at all: its delta says LONE.
 constexpr int FEW_KEYS = 16;
@@ -634,7 +637,7 @@ __device__ __forceinline__ void settle(f32x16 &ds, uint32_t bits)
 // dq of WAVES x 32 rows: the forward pass's walk over the keys, 32 keys at a time so that scores, their
 // gradients and the sums fit the registers of two waves a SIMD.  Three products a score; the walk that is
 // shared with dk and dv would save two of their seven and need atomic sums of dq, whose order changes
-// results.  The forward's window of 2048: 414-443 us; 8 x 12 x 1024 of 64: 38 us.
+// results.  The forward's window of 2048: 397-409 us; 8 x 12 x 1024 of 64: 38 us.
 template <int DT, int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a)
 {
@@ -701,13 +704,13 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 f32x16 s = zero16(), dp = zero16();
-    #pragma unroll
+#pragma unroll
                 for (int c = 0; c < C; c++) {
                     s = mma<DT>(Tile<HD>::rows(kt + n * (32 * Tile<HD>::ROW), rp, 0, c), q[c], s);
                     dp = mma<DT>(Tile<HD>::rows(vt + n * (32 * Tile<HD>::ROW), rp, 0, c), g[c], dp);
                 }
                 if (!whole) hide(s, bits);
-    #pragma unroll
+#pragma unroll
                 for (int r = 0; r < 16; r++) {
                     s[r] = exp2_hw(__builtin_fmaf(s[r], c2, -lse));
                     dp[r] = s[r] * (dp[r] - delta);
@@ -715,10 +718,10 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
                 if (!whole) settle(dp, bits);
                 lift.fit(dp, dq);
                 __builtin_amdgcn_sched_barrier(0);
-    #pragma unroll
+#pragma unroll
                 for (int k = 0; k < 2; k++) {
                     const u32x4 p = operand<DT>(dp, 8 * k);
-    #pragma unroll
+#pragma unroll
                     for (int d = 0; d < ND; d++) dq[d] = mma<DT>(Tile<HD>::columns(kt + n * (32 * Tile<HD>::ROW), cp, 16 * k, d), p, dq[d]);
                     if (!whole) {
                         const u32x4 rest = remainder<DT>(dp, 8 * k, p);
@@ -754,8 +757,9 @@ __global__ __launch_bounds__(WAVES * 64, HD == 64 ? 3 : 2) void attn_dq_kernel(A
 // workgroups of their own, and where there are few blocks each one's walk is cut into shares (DkvSplit);
 // the sums are fp32 partial results then.  Four products a score.  Heads of 128 hold k in registers and v
 // in LDS (both in registers spilled; separate kernels for dk and dv formed the scores twice and were slower
-// together).  The forward's window of 2048: 611 us, with the sinks' far positions in their block's own walk
-// 900; ragged fp16 sequences of few blocks 45 us and 7 to add their parts, in one walk each 109.
+// together).  The forward's window of 2048: 586-600 us, with the sinks' far positions in their block's own walk
+// 900; 8 x 12 x 1024 of 64: 61 us; ragged fp16 sequences of few blocks 50 us (46 without the powers of two) and 7 to
+// add their parts, in one walk each 109.
 template <int DT, int HD, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, DkvSplit cut)
 {
@@ -909,7 +913,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
                 for (int r = 0; r < 16; r += 4) {
                     const u32x4 po = *(const u32x4 *)(pos_s[side] + result_row(r, lane));
                     const f32x4 de = *(const f32x4 *)(delta_s[side] + result_row(r, lane));
-    #pragma unroll
+#pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const bool one = seen && sight.one((int)po[k], key);
                         bits |= ((uint32_t)one | (uint32_t)(one && !is_lone(de[k])) << 16) << (r + k);
@@ -918,16 +922,16 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
             }
             __builtin_amdgcn_sched_barrier(0);
             f32x16 s = zero16(), dp = zero16();
-    #pragma unroll
+#pragma unroll
             for (int c = 0; c < C; c++) {
                 s = mma<DT>(Tile<HD>::rows(qt, rp, 0, c), kf[c], s);
                 dp = mma<DT>(Tile<HD>::rows(gt, rp, 0, c), values(c), dp);
             }
             if (!whole) hide(s, bits);
-    #pragma unroll
+#pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const f32x4 ls = *(const f32x4 *)(lse_s[side] + result_row(r, lane)), de = *(const f32x4 *)(delta_s[side] + result_row(r, lane));
-    #pragma unroll
+#pragma unroll
                 for (int k = 0; k < 4; k++) {
                     s[r + k] = exp2_hw(__builtin_fmaf(s[r + k], c2, -ls[k]));
                     dp[r + k] = s[r + k] * (dp[r + k] - de[k]);
@@ -936,10 +940,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void attn_dkv_kernel(AttnArgs a, Dkv
             if (!whole) settle(dp, bits);
             lift.fit(dp, dk);
             __builtin_amdgcn_sched_barrier(0);
-    #pragma unroll
+#pragma unroll
             for (int k = 0; k < 2; k++) {
                 const u32x4 p = operand<DT>(s, 8 * k), ds = operand<DT>(dp, 8 * k);
-    #pragma unroll
+#pragma unroll
                 for (int d = 0; d < ND; d++) {
                     dv[d] = mma<DT>(Tile<HD>::columns(gt, cp, 16 * k, d), p, dv[d]);
                     dk[d] = mma<DT>(Tile<HD>::columns(qt, cp, 16 * k, d), ds, dk[d]);

@@ -9,10 +9,12 @@
 //
 // Bound by memory: N V logits read, and N V gradients written where they are asked for.  One
 // workgroup owns a row and keeps it in registers between the maximum, the sums and the gradient,
-// so that the logits are read once; a row too long for that is read again (from the last-level
-// cache, mostly).  8192 rows of 50257 bf16 with 64 entries each, gradient in place: 375 us, 4.4 TB/s of
-// the 1.65 GB read and written (a plain copy of that size reaches 4.8).  Rows start anywhere: the 16-byte pieces of a row are those of memory, and the
-// few elements before the first and behind the last whole piece go one by one.
+// so that the logits are read once; a row too long for that (over 102400 16-bit or 51200 fp32 logits) is read
+// again, three times in all: 4096 rows of 128256 bf16 827 us.  8192 rows of 50257 bf16 with 64 entries each, loss and
+// gradient: 362-373 us apart, 369 in place, 4.5 TB/s of the 1.65 GB read and written (a plain copy reaches 4.8); a T
+// without a short cut (3) costs no more.  Rows start anywhere: the 16-byte pieces of a row are those of memory, and
+// the few elements before the first and behind the last whole piece go one by one.
+
 #include <type_traits>
 
 #include "lm_common.h"
@@ -392,8 +394,8 @@ void go(const DistillArgs &a, hipStream_t stream)
 
 // How many threads hold a row, and how many of its pieces each.  With rows for every CU, few threads with
 // many registers: three rows of 512 threads and 13 pieces run on a CU, whose loads, sums and stores overlap
-// (8192 rows of 50257: 375 us; two of 14 pieces 425).  With fewer than two rows a CU, 1024 threads, which
-// bring one row in sooner (7 rows of 32000 fp32: loss 6.0 us, its gradient 6.8 us).
+// (8192 rows of 50257: 368 us; two of 14 pieces 425).  With fewer than two rows a CU, 1024 threads, which
+// bring one row in sooner (7 rows of 32000 fp32: loss 6.3 us, its gradient 6.9 us).
 template <int DT, int MODE>
 void pick(const DistillArgs &a, hipStream_t stream)
 {

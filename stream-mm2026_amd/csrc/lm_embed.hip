@@ -15,8 +15,8 @@
 //      tokens in registers.  A run inside its entries is final; the parts of a run that crosses
 //      the border go to fp32 partial rows.
 //   3. join: the wave that holds a crossing run's first entry adds its parts in order.
-// The gradient of 8192 tokens over 50257 x 768: 24-30 us for the sort and 131 MB of zeros, 12 and 4 us for
-// the rest; of 16384 tokens that favour few over 32000 x 4096 bf16: 34, 60 and 7 us.
+// The gradient of 8192 tokens over 50257 x 768: 23-30 us for the sort and 131 MB of zeros, 12 and 4 us for
+// the rest; of 16384 tokens that favour few over 32000 x 4096 bf16: 34, 61 and 8 us.
 #include "lm_common.h"
 #include "lm_embed.h"
 
@@ -36,7 +36,7 @@ __device__ __forceinline__ int64_t token_at(const void *tokens, int bytes, int64
 
 // ---------------------------------------------------------------- lookup
 // A workgroup takes whole rows, about 1024 pieces of VEC elements (blockIdx.y cuts longer rows): four
-// independent 16-byte loads a thread in flight.  8192 rows of 768 fp32: 10 us; 16384 rows of 4096 bf16
+// independent 16-byte loads a thread in flight.  8192 rows of 768 fp32: 11 us; 16384 rows of 4096 bf16
 // whose tokens favour few: 48 us, 5.6 TB/s of rows read and written (repeated rows come from cache).
 template <int WDT, int ODT, int VEC>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const void *tokens, int token_bytes, int64_t n, int64_t vocab, int dim,

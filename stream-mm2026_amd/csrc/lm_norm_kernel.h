@@ -15,8 +15,8 @@
 // too: loaded row by row they would be waited for behind the next row's (loads return in order).
 // Rows of up to 512 columns are one wave's, of up to 1024 two waves', longer ones a workgroup's.
 // Column sums stay in registers over all rows of a workgroup, then go to fp32 partial rows that a
-// second kernel adds in order (no float atomics).  16384 rows of 4096 bf16: forward 90 us (5.9 TB/s),
-// backward 169 us (4.8 TB/s, the rate of a large copy).
+// second kernel adds in order (no float atomics).  16384 rows of 4096 bf16: forward 92-97 us (5.7 TB/s),
+// backward 172-180 us (4.6 TB/s; a large copy reaches 4.8); 8192 of 768: 12 and 18 us.
 #pragma once
 #include "lm_common.h"
 #include "lm_norm.h"

@@ -373,6 +373,8 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
                        window: Optional[int] = 0, sinks: int = 0, scale: Optional[float] = None,
                        key_mask: Optional[torch.Tensor] = None, grads=None):
     """``(dq, dk, dv)`` from the forward call's tensors; those of shared key heads are summed in fp32.
+    Weights and score gradients are rounded to the tensors' type before their products (float16: scaled by
+    powers of two that keep them among its normal numbers).
 
     ``grads``: three tensors to write them into (views of one buffer, for a joint projection), with dense
     elements, 16-byte aligned rows and no overlap."""
