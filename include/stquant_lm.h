@@ -135,7 +135,8 @@ int stq_attention_backward(const stq_attention *a, void *stream);
  *   loss = alpha temperature^2 sum p (log p - log q) + (1 - alpha) (-log s[label])
  *   dlogits = drow (alpha temperature (q - p) + (1 - alpha) (s - [label]))
  * An entry whose id lies outside [0, vocab) is absent, a label outside it or a null `labels` too; a
- * row without entries has no first term, one without label no second, and one with neither is 0.
+ * row without entries has no first term, one without label no second, and one with neither is 0.  An
+ * entry with a weight whose logit lies more than 3.4e38 temperature below the row's largest gives an infinite loss.
  * logits, dlogits: [n, vocab] of one type, rows strided; dlogits may be logits itself.  teacher, ids:
  * [n, k] dense, 0 <= k <= 1024.  temperature: 1e-15 to 1e15; alpha: 0 to 1.  loss: [n] floats or null.  stats: [n, 4] floats.
  * forward: dlogits null: loss and stats; dlogits given: loss and dlogits from one read of the logits.
