@@ -1,6 +1,7 @@
 /*
  * stquant_lm.h -- C ABI of the transformer operators of libstquant_hip.so: embedding lookup,
- * residual norms, windowed attention and the distillation loss, each with its gradient.
+ * residual norms, windowed attention, the distillation loss, routing to experts, their products and
+ * the products' combination, each with its gradient, and the clipping of gradients to a global norm.
  *
  * Every call takes one argument struct (read before the call returns) and a hipStream_t, queues
  * its kernels on that stream and returns; nothing is allocated, copied or kept, so calls can be
@@ -20,7 +21,7 @@
 extern "C" {
 #endif
 
-#define STQ_LM_ABI_VERSION 1
+#define STQ_LM_ABI_VERSION 2
 
 /*
  * out[i, :] = scale * weight[tokens[i], :]; a token outside [0, vocab) gives a row of NaN.
@@ -161,6 +162,130 @@ typedef struct stq_distill {
 
 int stq_distill_forward(const stq_distill *a, void *stream);
 int stq_distill_backward(const stq_distill *a, void *stream);
+
+/*
+ * Routing: per row p = softmax(logits) over the experts, and the k largest logits, ties to the lowest
+ * expert; one of -inf is never chosen.  weights[j] = p of the j-th choice (renormalize: divided by the
+ * choices' sum), ids[j] its expert; a row with fewer than k choices ends with weight 0 and id -1.
+ * load[e] (or null) = sum of p[e] over the rows.  A row that holds a NaN or +inf has NaN for its p.
+ *   dlogits = p (dload - <p, dload> - [not renormalize] <weights, dweights>)
+ *           + [chosen] weights (dweights - [renormalize] <weights, dweights>)
+ * logits: [n, experts] rows strided, Float, BFloat16 or Half, dlogits the same type; the others dense floats and
+ * 32-bit ids.  experts 1 to 512, k 1 to min(experts, 64), n k up to 2^30.  dweights or dload may be null (zeros).
+ * backward reads weights and ids of the forward call.  workspace: forward with load, stq_route_workspace(a) bytes.
+ */
+typedef struct stq_route {
+    int64_t n, experts, k, dtype, renormalize;
+    const void *logits;
+    int64_t stride;
+    float *weights;
+    int32_t *ids;
+    float *load;
+    const float *dweights, *dload; /* backward */
+    void *dlogits;
+    int64_t dlogits_stride;
+    void *workspace;
+    int64_t workspace_bytes;
+} stq_route;
+
+int64_t stq_route_workspace(const stq_route *a);
+int stq_route_forward(const stq_route *a, void *stream);
+int stq_route_backward(const stq_route *a, void *stream);
+
+/*
+ * The slots sorted by expert, those of one expert in their order: rows[r] is the slot at place r, places[s]
+ * where slot s stands, and expert e owns the places offsets[e] to offsets[e + 1] (experts + 1 offsets).  Slots
+ * whose id lies outside [0, experts) come last.  slots up to 2^30, experts 1 to 512.
+ */
+typedef struct stq_expert_plan {
+    const void *ids; /* [slots], STQ_LONG or STQ_INT */
+    int64_t id_dtype, slots, experts;
+    int32_t *rows, *places, *offsets;
+    void *workspace;
+    int64_t workspace_bytes;
+} stq_expert_plan;
+
+int64_t stq_expert_plan_workspace(const stq_expert_plan *a);
+int stq_expert_plan_sort(const stq_expert_plan *a, void *stream);
+
+/*
+ * Products of each expert's run of rows with its weight [out, in]:
+ *   y[r, :] = W[e] x[r, :],  dx[r, :] = W[e]^T dy[r, :],  dW[e] = sum over its rows of dy[r, :] x[r, :]^T
+ * k > 0: row r reads x[rows[r] / k] of the `tokens` = slots / k rows of x, and dx is the sum over a token's k rows
+ * (in fp32, rounded once); k = 0: row r is row r of x and dx.  Rows of no expert give y = dx = 0 and add nothing to dW,
+ * an expert without rows gets dW = 0.  Sums are fp32, results rounded once.
+ * BFloat16 or Half; in and out multiples of 8 up to 2^20; x, weight, dy: rows strided, 16-byte aligned, strides multiples
+ * of 8; y, dx, dweight dense and aligned likewise.  dweight_dtype: dtype or Float.  backward: dx or dweight may be null (not wanted).
+ * slots up to 2^30, and slots / 128 + experts times the tiles of 128 of the wider of in and out up to 2^23.
+ * workspace: backward with dx and k > 0, stq_expert_product_workspace(a) bytes.
+ */
+typedef struct stq_expert_product {
+    int64_t dtype, slots, experts, in, out, k, tokens;
+    const void *x;
+    int64_t x_stride;
+    const void *weight;
+    int64_t weight_expert_stride, weight_row_stride;
+    const int32_t *rows, *places, *offsets; /* of a plan; rows and places with k > 0 */
+    void *y;
+    const void *dy; /* backward */
+    int64_t dy_stride;
+    void *dx, *dweight;
+    int64_t dweight_dtype;
+    void *workspace;
+    int64_t workspace_bytes;
+} stq_expert_product;
+
+int64_t stq_expert_product_workspace(const stq_expert_product *a);
+int stq_expert_product_forward(const stq_expert_product *a, void *stream);
+int stq_expert_product_backward(const stq_expert_product *a, void *stream);
+
+/*
+ * out[t, :] = sum over j of weights[t, j] y[places[t, j], :] in fp32, slots of no expert left out (weights null: ones).
+ *   dy[places[t, j], :] = weights[t, j] dout[t, :] (0 for slots of no expert),  dweights[t, j] = <y[places[t, j], :], dout[t, :]>
+ * Float, BFloat16 or Half; y and dout rows strided, the others dense.  k 1 to 64, n k up to 2^30, dim up to 2^24.
+ * dweights null: not wanted (y is then not read).
+ */
+typedef struct stq_expert_combine {
+    int64_t n, k, experts, dim, dtype;
+    const void *y;
+    int64_t y_stride;
+    const float *weights;
+    const int32_t *places, *offsets;
+    void *out;
+    const void *dout; /* backward */
+    int64_t dout_stride;
+    void *dy;
+    float *dweights;
+} stq_expert_combine;
+
+int stq_expert_combine_forward(const stq_expert_combine *a, void *stream);
+int stq_expert_combine_backward(const stq_expert_combine *a, void *stream);
+
+/*
+ * The 2-norm of all tensors together, and out = grad min(1, max_norm / (norm + 1e-6)), of which a NaN norm makes NaN and
+ * an infinite one 0 (NaN where the gradient is infinite).  Squares are added in double.  norm: one float on the
+ * device.  given (or null): a norm to scale by in place of theirs, e.g. one summed over ranks; norm is then not written.
+ * out may be grad; otherwise it lies apart from every grad and out of the list.  numel up to 2^40.
+ * workspace: stq_clip_workspace(a) bytes, 16-byte aligned.  The list is read before the call returns.
+ */
+typedef struct stq_grad {
+    const void *grad; /* dense, Float, BFloat16 or Half */
+    void *out; /* the same type; not read by stq_grad_norm */
+    int64_t numel, dtype;
+} stq_grad;
+typedef struct stq_clip {
+    const stq_grad *grads;
+    int64_t count;
+    double max_norm; /* >= 0 */
+    const float *given;
+    float *norm;
+    void *workspace;
+    int64_t workspace_bytes;
+} stq_clip;
+
+int64_t stq_clip_workspace(const stq_clip *a);
+int stq_grad_norm(const stq_clip *a, void *stream);
+int stq_clip_grads(const stq_clip *a, void *stream);
 
 /* STQ_LM_ABI_VERSION the library was built with. */
 int stq_lm_abi_version(void);

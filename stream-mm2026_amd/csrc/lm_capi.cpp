@@ -2,15 +2,20 @@
 // checks and the launches' arguments.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
+#include <new>
+#include <vector>
 
 #include "../../include/stquant_hip.h"
 #include "../../include/stquant_lm.h"
 #include "lm_attn.h"
+#include "lm_clip.h"
 #include "lm_common.h"
 #include "lm_distill.h"
 #include "lm_embed.h"
+#include "lm_expert.h"
 #include "lm_norm.h"
 #include "mdq_error.h"
 
@@ -306,6 +311,258 @@ lm::DistillArgs distill_args(const stq_distill *a)
     return o;
 }
 
+int check_workspace(const void *p, int64_t bytes, int64_t need)
+{
+    if (need) CHECK(check_ptr("workspace", p, 16));
+    if (bytes < need)
+        return fail(STQ_ERR_INVALID, "workspace needs %lld bytes, got %lld", (long long)need, (long long)bytes);
+    return STQ_OK;
+}
+
+// The sizes alone (what the workspaces follow from).
+int check_route_sizes(const stq_route *a)
+{
+    if (!a) return bad("null arguments");
+    if (!is_float(a->dtype)) return bad_type("logits", a->dtype, FLOATS);
+    CHECK(check_size("experts", a->experts, 1, lm::EXPERT_MAX));
+    CHECK(check_size("k", a->k, 1, a->experts < lm::ROUTE_MAX_K ? a->experts : lm::ROUTE_MAX_K));
+    return check_size("n", a->n, 0, lm::SLOT_MAX / a->k);
+}
+
+int check_route(const stq_route *a, bool backward)
+{
+    CHECK(check_route_sizes(a));
+    if (a->renormalize != 0 && a->renormalize != 1) return bad("renormalize must be 0 or 1");
+    if (!backward && a->load) {
+        CHECK(check_ptr("load", a->load, 4));
+        CHECK(check_workspace(a->workspace, a->workspace_bytes, lm::route_workspace(a->n, (int)a->experts)));
+    }
+    if (a->n == 0) return STQ_OK;
+    CHECK(check_ptr("logits", a->logits, size_of(a->dtype)));
+    if (a->stride < 0) return bad("rows of logits: the stride must be >= 0");
+    CHECK(check_ptr("weights", a->weights, 4));
+    CHECK(check_ptr("ids", a->ids, 4));
+    if (!backward) return STQ_OK;
+    if (a->dweights) CHECK(check_ptr("dweights", a->dweights, 4));
+    if (a->dload) CHECK(check_ptr("dload", a->dload, 4));
+    CHECK(check_ptr("dlogits", a->dlogits, size_of(a->dtype)));
+    if (a->dlogits_stride < a->experts) return bad("rows of dlogits must not overlap");
+    return STQ_OK;
+}
+
+lm::RouteArgs route_args(const stq_route *a)
+{
+    lm::RouteArgs o;
+    o.logits = a->logits;
+    o.dt = (int)a->dtype;
+    o.n = a->n;
+    o.stride = a->stride;
+    o.experts = (int)a->experts;
+    o.k = (int)a->k;
+    o.renormalize = (int)a->renormalize;
+    o.weights = a->weights;
+    o.ids = a->ids;
+    o.load = a->load;
+    o.partial = (float *)a->workspace;
+    o.dweights = a->dweights;
+    o.dload = a->dload;
+    o.dlogits = a->dlogits;
+    o.dstride = a->dlogits_stride;
+    return o;
+}
+
+int check_plan_sizes(const stq_expert_plan *a)
+{
+    if (!a) return bad("null arguments");
+    if (!is_index(a->id_dtype)) return bad_type("ids", a->id_dtype, INDEXES);
+    CHECK(check_size("experts", a->experts, 1, lm::EXPERT_MAX));
+    return check_size("slots", a->slots, 0, lm::SLOT_MAX);
+}
+
+// Rows of 16-byte pieces.
+int check_pieces(const char *name, const void *p, int64_t stride)
+{
+    CHECK(check_ptr(name, p, 16));
+    if (stride < 0 || stride % 8) return fail(STQ_ERR_INVALID, "%s: strides must be multiples of 8 elements, >= 0", name);
+    return STQ_OK;
+}
+
+int check_product_sizes(const stq_expert_product *a)
+{
+    if (!a) return bad("null arguments");
+    if (a->dtype != STQ_BFLOAT16 && a->dtype != STQ_HALF) return bad_type("x and weight", a->dtype, "BFloat16 or Half");
+    CHECK(check_size("experts", a->experts, 1, lm::EXPERT_MAX));
+    CHECK(check_size("slots", a->slots, 0, lm::SLOT_MAX));
+    CHECK(check_size("in", a->in, 8, 1 << 20));
+    CHECK(check_size("out", a->out, 8, 1 << 20));
+    if (a->in % 8 || a->out % 8) return bad("in and out must be multiples of 8");
+    CHECK(check_size("k", a->k, 0, lm::ROUTE_MAX_K));
+    if (a->k) CHECK(check_size("tokens", a->tokens, 0, lm::SLOT_MAX));
+    if (a->k && a->tokens * a->k != a->slots)
+        return fail(STQ_ERR_INVALID, "slots (%lld) must be tokens (%lld) times k (%lld)", (long long)a->slots, (long long)a->tokens, (long long)a->k);
+    // (a launch has fewer than 2^32 threads along a dimension)
+    const int64_t wide = ((a->in > a->out ? a->in : a->out) + 127) / 128, narrow = ((a->in > a->out ? a->out : a->in) + 127) / 128;
+    CHECK(check_size("tiles of rows", (a->slots / 128 + a->experts + 1) * wide, 0, 1 << 23));
+    return check_size("tiles of weights", a->experts * wide * narrow, 0, 1 << 23);
+}
+
+int check_product(const stq_expert_product *a, bool backward)
+{
+    CHECK(check_product_sizes(a));
+    CHECK(check_ptr("offsets", a->offsets, 4));
+    CHECK(check_ptr("weight", a->weight, 16));
+    if (a->weight_expert_stride % 8 || a->weight_row_stride % 8 || a->weight_expert_stride < 0 || a->weight_row_stride < 0)
+        return bad("weight: strides must be multiples of 8 elements, >= 0");
+    if (a->slots) {
+        if (a->k) {
+            CHECK(check_ptr("rows", a->rows, 4));
+            CHECK(check_ptr("places", a->places, 4));
+        }
+        CHECK(check_pieces("x", a->x, a->x_stride));
+        if (backward) CHECK(check_pieces("dy", a->dy, a->dy_stride));
+        else CHECK(check_ptr("y", a->y, 16));
+        if (backward && a->dx) CHECK(check_ptr("dx", a->dx, 16));
+    }
+    if (backward && a->dweight) {
+        if (a->dweight_dtype != a->dtype && a->dweight_dtype != STQ_FLOAT) return bad_type("dweight", a->dweight_dtype, "Float or the type of x");
+        CHECK(check_ptr("dweight", a->dweight, 16));
+    }
+    return STQ_OK;
+}
+
+lm::ProductArgs product_args(const stq_expert_product *a)
+{
+    lm::ProductArgs o;
+    o.slots = a->slots;
+    o.experts = (int)a->experts;
+    o.in = (int)a->in;
+    o.out = (int)a->out;
+    o.k = (int)a->k;
+    o.tokens = a->tokens;
+    o.x = a->x;
+    o.x_stride = a->x_stride;
+    o.weight = a->weight;
+    o.weight_expert_stride = a->weight_expert_stride;
+    o.weight_row_stride = a->weight_row_stride;
+    o.y = a->y;
+    o.rows = a->rows;
+    o.places = a->places;
+    o.offsets = a->offsets;
+    o.dy = a->dy;
+    o.dy_stride = a->dy_stride;
+    o.dx = a->dx;
+    o.scratch = a->k ? (float *)a->workspace : nullptr;
+    o.dweight = a->dweight;
+    o.dweight_f32 = a->dweight_dtype == STQ_FLOAT;
+    return o;
+}
+
+int check_combine(const stq_expert_combine *a, bool backward)
+{
+    if (!a) return bad("null arguments");
+    if (!is_float(a->dtype)) return bad_type("y", a->dtype, FLOATS);
+    CHECK(check_size("experts", a->experts, 1, lm::EXPERT_MAX));
+    CHECK(check_size("k", a->k, 1, lm::ROUTE_MAX_K));
+    CHECK(check_size("n", a->n, 0, lm::SLOT_MAX / a->k));
+    CHECK(check_size("dim", a->dim, 1, 1 << 24));
+    if (a->n == 0) return STQ_OK;
+    const int z = size_of(a->dtype);
+    if (a->weights) CHECK(check_ptr("weights", a->weights, 4));
+    CHECK(check_ptr("places", a->places, 4));
+    CHECK(check_ptr("offsets", a->offsets, 4));
+    if (!backward || a->dweights) {
+        CHECK(check_ptr("y", a->y, z));
+        if (a->y_stride < 0) return bad("y_stride must be >= 0");
+    }
+    if (!backward) return check_ptr("out", a->out, z);
+    CHECK(check_ptr("dout", a->dout, z));
+    if (a->dout_stride < 0) return bad("dout_stride must be >= 0");
+    if (a->dweights) CHECK(check_ptr("dweights", a->dweights, 4));
+    return check_ptr("dy", a->dy, z);
+}
+
+lm::CombineArgs combine_args(const stq_expert_combine *a)
+{
+    lm::CombineArgs o;
+    o.n = a->n;
+    o.k = (int)a->k;
+    o.experts = (int)a->experts;
+    o.dim = a->dim;
+    o.y = a->y;
+    o.y_dt = o.out_dt = (int)a->dtype;
+    o.y_stride = a->y_stride;
+    o.weights = a->weights;
+    o.places = a->places;
+    o.offsets = a->offsets;
+    o.out = a->out;
+    o.out_stride = a->dim;
+    o.dout = a->dout;
+    o.dout_stride = a->dout_stride;
+    o.dy = a->dy;
+    o.dweights = a->dweights;
+    return o;
+}
+
+int check_clip_list(const stq_clip *a)
+{
+    if (!a) return bad("null arguments");
+    CHECK(check_size("count", a->count, 0, 1 << 24));
+    if (a->count && !a->grads) return bad("grads: null data pointer");
+    for (int64_t i = 0; i < a->count; i++) {
+        const stq_grad &g = a->grads[i];
+        if (!is_float(g.dtype)) return bad_type("gradients", g.dtype, FLOATS);
+        CHECK(check_size("elements of a gradient", g.numel, 0, (int64_t)1 << 40));
+        if (g.numel) CHECK(check_ptr("grad", g.grad, size_of(g.dtype)));
+    }
+    return STQ_OK;
+}
+
+// What is written lies apart from everything else in the list, but for a gradient in place.
+int check_clip_apart(const stq_clip *a)
+{
+    struct Span {
+        const char *from, *to;
+        int64_t of;                       // the tensor; < 0: written, ~tensor
+    };
+    std::vector<Span> spans;
+    spans.reserve(2 * a->count);
+    for (int64_t i = 0; i < a->count; i++) {
+        const stq_grad &g = a->grads[i];
+        if (g.numel == 0) continue;
+        CHECK(check_ptr("out", g.out, size_of(g.dtype)));
+        const int64_t bytes = g.numel * size_of(g.dtype);
+        spans.push_back({(const char *)g.out, (const char *)g.out + bytes, ~i});
+        if (g.out != g.grad) spans.push_back({(const char *)g.grad, (const char *)g.grad + bytes, i});
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span &x, const Span &y) { return x.from < y.from; });
+    // the farthest ends so far, of all spans and of those written
+    const char *any = nullptr, *written = nullptr;
+    for (const Span &s : spans) {
+        if ((s.of < 0 && any > s.from) || written > s.from) return bad("gradients that are written must not overlap others");
+        any = std::max(any, s.to);
+        if (s.of < 0) written = std::max(written, s.to);
+    }
+    return STQ_OK;
+}
+
+std::vector<lm::ClipTensor> clip_tensors(const stq_clip *a)
+{
+    std::vector<lm::ClipTensor> t(a->count);
+    for (int64_t i = 0; i < a->count; i++) t[i] = {a->grads[i].grad, a->grads[i].out, a->grads[i].numel, (int)a->grads[i].dtype};
+    return t;
+}
+
+// No exception leaves a C entry.
+template <typename F>
+auto guarded(F f, decltype(f()) failed) -> decltype(f())
+{
+    try {
+        return f();
+    } catch (const std::bad_alloc &) {
+        return bad("out of host memory"), failed;
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -429,6 +686,120 @@ int stq_distill_backward(const stq_distill *a, void *stream)
     CHECK(check_ptr("stats", a->stats, 4));
     if (!a->dlogits) return bad("dlogits: null data pointer");
     return done(lm::distill_backward(distill_args(a), (hipStream_t)stream), "distill backward");
+}
+
+int64_t stq_route_workspace(const stq_route *a)
+{
+    if (check_route_sizes(a) != STQ_OK) return -1;
+    return lm::route_workspace(a->n, (int)a->experts);
+}
+
+int stq_route_forward(const stq_route *a, void *stream)
+{
+    CHECK(check_route(a, false));
+    if (a->n == 0 && !a->load) return STQ_OK;
+    return done(lm::route_forward(route_args(a), (hipStream_t)stream), "route forward");
+}
+
+int stq_route_backward(const stq_route *a, void *stream)
+{
+    CHECK(check_route(a, true));
+    if (a->n == 0) return STQ_OK;
+    return done(lm::route_backward(route_args(a), (hipStream_t)stream), "route backward");
+}
+
+int64_t stq_expert_plan_workspace(const stq_expert_plan *a)
+{
+    if (check_plan_sizes(a) != STQ_OK) return -1;
+    return lm::plan_workspace(a->slots, (int)a->experts);
+}
+
+int stq_expert_plan_sort(const stq_expert_plan *a, void *stream)
+{
+    CHECK(check_plan_sizes(a));
+    CHECK(check_ptr("offsets", a->offsets, 4));
+    if (a->slots) {
+        CHECK(check_ptr("ids", a->ids, size_of(a->id_dtype)));
+        CHECK(check_ptr("rows", a->rows, 4));
+        CHECK(check_ptr("places", a->places, 4));
+    }
+    CHECK(check_workspace(a->workspace, a->workspace_bytes, lm::plan_workspace(a->slots, (int)a->experts)));
+    const lm::PlanArgs p = {a->ids, size_of(a->id_dtype), a->slots, (int)a->experts, a->rows, a->places, a->offsets, (int32_t *)a->workspace};
+    return done(lm::expert_plan(p, (hipStream_t)stream), "expert plan");
+}
+
+int64_t stq_expert_product_workspace(const stq_expert_product *a)
+{
+    if (check_product_sizes(a) != STQ_OK) return -1;
+    return lm::product_workspace(product_args(a));
+}
+
+int stq_expert_product_forward(const stq_expert_product *a, void *stream)
+{
+    CHECK(check_product(a, false));
+    if (a->slots == 0) return STQ_OK;
+    const lm::ProductArgs o = product_args(a);
+    return done(a->dtype == STQ_BFLOAT16 ? lm::product_forward<lm::DT_BF16>(o, (hipStream_t)stream) : lm::product_forward<lm::DT_F16>(o, (hipStream_t)stream),
+                "expert product forward");
+}
+
+int stq_expert_product_backward(const stq_expert_product *a, void *stream)
+{
+    CHECK(check_product(a, true));
+    lm::ProductArgs o = product_args(a);
+    if (a->slots == 0) o.dx = nullptr;
+    CHECK(check_workspace(a->workspace, a->workspace_bytes, lm::product_workspace(o)));
+    return done(a->dtype == STQ_BFLOAT16 ? lm::product_backward<lm::DT_BF16>(o, (hipStream_t)stream) : lm::product_backward<lm::DT_F16>(o, (hipStream_t)stream),
+                "expert product backward");
+}
+
+int stq_expert_combine_forward(const stq_expert_combine *a, void *stream)
+{
+    CHECK(check_combine(a, false));
+    return done(lm::combine_forward(combine_args(a), (hipStream_t)stream), "expert combine forward");
+}
+
+int stq_expert_combine_backward(const stq_expert_combine *a, void *stream)
+{
+    CHECK(check_combine(a, true));
+    return done(lm::combine_backward(combine_args(a), (hipStream_t)stream), "expert combine backward");
+}
+
+int64_t stq_clip_workspace(const stq_clip *a)
+{
+    return guarded([&]() -> int64_t {
+        if (check_clip_list(a) != STQ_OK) return -1;
+        const auto t = clip_tensors(a);
+        return lm::clip_workspace(t.data(), (int64_t)t.size());
+    }, -1);
+}
+
+int stq_grad_norm(const stq_clip *a, void *stream)
+{
+    return guarded([&]() -> int {
+        CHECK(check_clip_list(a));
+        CHECK(check_ptr("norm", a->norm, 4));
+        const auto t = clip_tensors(a);
+        CHECK(check_workspace(a->workspace, a->workspace_bytes, lm::clip_workspace(t.data(), (int64_t)t.size())));
+        return done(lm::clip_norm(t.data(), (int64_t)t.size(), (double *)a->workspace, a->norm, (hipStream_t)stream), "gradient norm");
+    }, STQ_ERR_INVALID);
+}
+
+int stq_clip_grads(const stq_clip *a, void *stream)
+{
+    return guarded([&]() -> int {
+        CHECK(check_clip_list(a));
+        if (!(a->max_norm >= 0.0)) return bad("max_norm must be >= 0");
+        CHECK(check_clip_apart(a));
+        const auto t = clip_tensors(a);
+        if (a->given) CHECK(check_ptr("given norm", a->given, 4));
+        else {
+            CHECK(check_ptr("norm", a->norm, 4));
+            CHECK(check_workspace(a->workspace, a->workspace_bytes, lm::clip_workspace(t.data(), (int64_t)t.size())));
+        }
+        return done(lm::clip_scale(t.data(), (int64_t)t.size(), a->max_norm, a->given, (double *)a->workspace, a->given ? nullptr : a->norm, (hipStream_t)stream),
+                    "gradient clipping");
+    }, STQ_ERR_INVALID);
 }
 
 }  // extern "C"

@@ -68,9 +68,22 @@ LM_SYMBOLS = (
     "stq_attention_backward",
     "stq_distill_forward",
     "stq_distill_backward",
+    "stq_route_workspace",
+    "stq_route_forward",
+    "stq_route_backward",
+    "stq_expert_plan_workspace",
+    "stq_expert_plan_sort",
+    "stq_expert_product_workspace",
+    "stq_expert_product_forward",
+    "stq_expert_product_backward",
+    "stq_expert_combine_forward",
+    "stq_expert_combine_backward",
+    "stq_clip_workspace",
+    "stq_grad_norm",
+    "stq_clip_grads",
     "stq_lm_abi_version",
 )
-LM_ABI_VERSION = 1
+LM_ABI_VERSION = 2
 
 # STQ_ABI_VERSION of include/stquant_hip.h this package is written against
 ABI_VERSION = 4

@@ -6,6 +6,11 @@ What a training step runs around the optimizer, each with its gradient:
 ``norm_residual``  the norms before and after a block, fused with its gate and the residual sum
 ``attention``      causal attention over a window of the last keys and a few first ones (sinks)
 ``distill_loss``   learning from a teacher's top logits, mixed with the labels' cross-entropy
+``route``          softmax over experts, each token's top k of them, and how they are loaded
+``expert_plan``    the tokens' slots sorted by expert
+``expert_product`` each expert's weight times its own run of rows
+``expert_combine`` the weighted sum of what a token's experts gave
+``clip_grads``     all gradients scaled to a global norm, ahead of the optimizer's step
 
 The plain names are differentiable (``torch.autograd``), once: a second derivative raises.  The
 ``*_forward`` / ``*_backward`` pairs and ``distill_loss_and_grad`` are the calls beneath them, for
@@ -18,10 +23,11 @@ tensors' type, and the same call gives the same bits every time.
 """
 from __future__ import annotations
 
+import ctypes
 import os
 import struct
 import sys
-from typing import Optional
+from typing import Iterable, NamedTuple, Optional
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -38,6 +44,10 @@ __all__ = [
     "norm_residual", "norm_residual_forward", "norm_residual_backward",
     "attention", "attention_forward", "attention_backward",
     "distill_loss", "distill_loss_forward", "distill_loss_backward", "distill_loss_and_grad",
+    "route", "route_forward", "route_backward", "ExpertPlan", "expert_plan",
+    "expert_product", "expert_product_forward", "expert_product_backward",
+    "expert_combine", "expert_combine_forward", "expert_combine_backward",
+    "grad_norm", "clip_grads",
 ]
 
 _FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -48,6 +58,11 @@ _EMBED_GRAD = struct.Struct("@Qqqqq Qqq Qqq qq Qq d")
 _NORM = struct.Struct("@4q 2Q2q 5Q 2q 2d 3Q 2Q2q 7Q Qq")
 _ATTN = struct.Struct("@9q d 4q4q4q4q Qq Q 4q4q4q4q Qq")
 _DISTILL = struct.Struct("@3q Qq Qq Qqq Qq 2d 2Q Q Qq")
+_ROUTE = struct.Struct("@5q Qq 3Q 2Q Qq Qq")
+_PLAN = struct.Struct("@Q3q 3Q Qq")
+_PRODUCT = struct.Struct("@7q Qq Qqq 3Q Q Qq 2Q q Qq")
+_COMBINE = struct.Struct("@5q Qq Q 2Q Q Qq 2Q")
+_CLIP = struct.Struct("@Qq d 2Q Qq")
 
 
 def _fail(msg: str):
@@ -543,3 +558,340 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids
                  temperature: float = 1.0, alpha: float = 1.0) -> torch.Tensor:
     """``loss`` of :func:`distill_loss_forward` ([...], fp32), differentiable in ``logits``."""
     return _DistillLoss.apply(logits, teacher_logits, teacher_ids, labels, temperature, alpha)
+
+
+# ---------------------------------------------------------------- routing to experts
+def _route_args(logits, k):
+    """The checked logits as rows, and the struct's leading fields but for renormalize."""
+    zc = _float_code("logits", logits)
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        _fail(f"logits must be [..., experts], got {tuple(logits.shape)}")
+    _same_device(logits)
+    z = _rows(logits, logits.shape[-1])
+    return z, (z.shape[0], z.shape[1], int(k), zc)
+
+
+def route_forward(logits: torch.Tensor, k: int, *, renormalize: bool = False):
+    """``(weights, ids, load)``: each row's ``k`` experts of the largest logits and their probabilities.
+
+    ``logits`` [..., experts] (up to 512).  With p the softmax of a row, ``weights`` [..., k] (fp32) are p of
+    the chosen experts, largest first, or with ``renormalize`` their shares of the chosen ones' sum; ``ids`` [..., k]
+    (int32) the experts, equal logits by the lowest.  An expert of logit -inf is never chosen: a row with fewer
+    than ``k`` others ends with weight 0 and id -1, one of -inf throughout (padding) chooses none.  ``load``
+    [experts] (fp32) is the sum of p over the rows, from which a loss for balance is formed."""
+    z, head = _route_args(logits, k)
+    lead = logits.shape[:-1]
+    weights = torch.empty((*lead, head[2]), dtype=torch.float32, device=z.device)
+    ids = torch.empty((*lead, head[2]), dtype=torch.int32, device=z.device)
+    load = torch.empty((head[1],), dtype=torch.float32, device=z.device)
+    args = [*head, int(renormalize), z.data_ptr(), z.stride(0), weights.data_ptr(), ids.data_ptr(), load.data_ptr(), *(0,) * 6]
+    L = lm_lib()
+    ws = _workspace(_size(L.stq_route_workspace, _ROUTE.pack(*args)), z.device)
+    args[-2:] = ws.data_ptr(), ws.numel()
+    _call(z.device, L.stq_route_forward, _ROUTE.pack(*args))
+    return weights, ids, load
+
+
+def route_backward(dweights: Optional[torch.Tensor], dload: Optional[torch.Tensor], logits: torch.Tensor, weights: torch.Tensor,
+                   ids: torch.Tensor, *, renormalize: bool = False) -> torch.Tensor:
+    """The gradient of the logits (their type) from those of ``weights`` and ``load`` (fp32; None: zeros) and the
+    forward call's tensors."""
+    z, head = _route_args(logits, ids.shape[-1] if ids.dim() else 0)
+    shape = (*logits.shape[:-1], head[2])
+    for name, t, want, dtype in (("weights", weights, shape, torch.float32), ("ids", ids, shape, torch.int32),
+                                 ("dweights", dweights, shape, torch.float32), ("dload", dload, (head[1],), torch.float32)):
+        if t is not None and (t.shape != want or t.dtype != dtype):
+            _fail(f"{name} must be {tuple(want)} of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    _same_device(z, weights=weights, ids=ids, dweights=dweights, dload=dload)
+    weights, ids = weights.contiguous(), ids.contiguous()
+    dweights, dload = (None if t is None else t.contiguous() for t in (dweights, dload))
+    dz = torch.empty(logits.shape, dtype=logits.dtype, device=z.device)
+    _call(z.device, lm_lib().stq_route_backward,
+          _ROUTE.pack(*head, int(renormalize), z.data_ptr(), z.stride(0), weights.data_ptr(), ids.data_ptr(), 0, _ptr(dweights), _ptr(dload),
+                      dz.data_ptr(), z.shape[1], 0, 0))
+    return dz
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, renormalize):
+        weights, ids, load = route_forward(logits, k, renormalize=renormalize)
+        ctx.save_for_backward(logits, weights, ids)
+        ctx.renormalize = renormalize
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        return weights, ids, load
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dweights, dids, dload):
+        logits, weights, ids = ctx.saved_tensors
+        return route_backward(dweights, dload, logits, weights, ids, renormalize=ctx.renormalize), None, None
+
+
+def route(logits: torch.Tensor, k: int, *, renormalize: bool = False):
+    """``(weights, ids, load)`` of :func:`route_forward`, weights and load differentiable in ``logits``."""
+    return _Route.apply(logits, k, renormalize)
+
+
+class ExpertPlan(NamedTuple):
+    """Slots (a token's choices) sorted by expert, int32 and dense: ``rows`` [slots] the slot at each place, ``places``
+    [..., k] where each slot stands, ``offsets`` [experts + 1]: expert e owns places offsets[e] to offsets[e + 1].
+    Slots of no expert stand behind the last offset."""
+    rows: torch.Tensor
+    places: torch.Tensor
+    offsets: torch.Tensor
+
+
+def expert_plan(ids: torch.Tensor, experts: int) -> ExpertPlan:
+    """The slots of ``ids`` [..., k] sorted by expert, those of one expert in their order.  Ids outside
+    [0, experts) (-1) belong to none."""
+    ic = _index_code("ids", ids)
+    if ids.dim() < 1:
+        _fail("ids must be [..., k]")
+    _same_device(ids)
+    ids = ids.contiguous()
+    n = ids.numel()
+    rows = torch.empty((n,), dtype=torch.int32, device=ids.device)
+    places = torch.empty(ids.shape, dtype=torch.int32, device=ids.device)
+    offsets = torch.empty((max(int(experts), 0) + 1,), dtype=torch.int32, device=ids.device)
+    args = [ids.data_ptr(), ic, n, int(experts), rows.data_ptr(), places.data_ptr(), offsets.data_ptr(), 0, 0]
+    L = lm_lib()
+    ws = _workspace(_size(L.stq_expert_plan_workspace, _PLAN.pack(*args)), ids.device)
+    if ws is not None:
+        args[-2:] = ws.data_ptr(), ws.numel()
+    _call(ids.device, L.stq_expert_plan_sort, _PLAN.pack(*args))
+    return ExpertPlan(rows, places, offsets)
+
+
+def _check_plan(plan: ExpertPlan, near: torch.Tensor) -> None:
+    rows, places, offsets = plan
+    for name, t in (("rows", rows), ("places", places), ("offsets", offsets)):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            _fail(f"the plan's {name} must be dense int32, got {t.dtype}")
+    if places.dim() < 1 or rows.shape != (places.numel(),) or offsets.dim() != 1 or offsets.numel() < 2:
+        _fail(f"not a plan: rows {tuple(rows.shape)}, places {tuple(places.shape)}, offsets {tuple(offsets.shape)}")
+    _same_device(near, rows=rows, places=places, offsets=offsets)
+
+
+def _pieces(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with dense rows that begin on 16 bytes (a copy if they do not)."""
+    s = t.stride()
+    if (s[-1] == 1 or t.shape[-1] == 1) and not any(x % 8 for x in s[:-1]) and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _product_args(x, weight, plan, gather):
+    """The checked operands as the kernels read them, and the struct's leading fields."""
+    if weight.dim() != 3:
+        _fail(f"weight must be [experts, out, in], got {tuple(weight.shape)}")
+    if x.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != x.dtype:
+        _fail(f"x and weight must both be bfloat16 or both float16, got {x.dtype} and {weight.dtype}")
+    _check_plan(plan, x)
+    _same_device(x, weight=weight)
+    experts, out, width = weight.shape
+    slots, lead = plan.rows.numel(), plan.places.shape[:-1] if gather else plan.rows.shape
+    if x.shape != (*lead, width):
+        _fail(f"x must be {(*lead, width)}, got {tuple(x.shape)}")
+    if plan.offsets.numel() != experts + 1:
+        _fail(f"the plan is for {plan.offsets.numel() - 1} experts, weight has {experts}")
+    xr, w = _pieces(_rows(x, width)), _pieces(weight)
+    head = (_FLOATS[x.dtype], slots, experts, width, out, plan.places.shape[-1] if gather else 0, xr.shape[0], xr.data_ptr(), xr.stride(0),
+            w.data_ptr(), w.stride(0), w.stride(1), plan.rows.data_ptr(), plan.places.data_ptr(), plan.offsets.data_ptr())
+    return (xr, w), head
+
+
+def expert_product_forward(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *, gather: bool = False) -> torch.Tensor:
+    """``y`` [slots, out]: the row at each place of the plan times the weight of the expert that owns it, ``x W[e]^T``.
+
+    ``weight`` [experts, out, in]; ``x`` [slots, in] in the plan's order, or with ``gather`` the tokens
+    [..., in] whose choices the plan sorted, each read wherever one of its slots stands.  Rows of no expert are 0.
+    bfloat16 or float16, in and out multiples of 8; sums are fp32, rounded once."""
+    keep, head = _product_args(x, weight, plan, gather)
+    y = torch.empty((plan.rows.numel(), weight.shape[1]), dtype=x.dtype, device=x.device)
+    _call(x.device, lm_lib().stq_expert_product_forward, _PRODUCT.pack(*head, y.data_ptr(), *(0,) * 7))
+    return y
+
+
+def expert_product_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *, gather: bool = False,
+                            inputs: bool = True, weights: bool = True, dtype: Optional[torch.dtype] = None):
+    """``(dx, dweight)``: the gradients of ``x`` (with ``gather`` summed over a token's slots in fp32) and of ``weight``, in
+    ``dtype`` (its own type or float32); None for what ``inputs`` or ``weights`` leaves out.  An expert without rows gets zeros."""
+    keep, head = _product_args(x, weight, plan, gather)
+    want = (plan.rows.numel(), weight.shape[1])
+    if dy.shape != want or dy.dtype != x.dtype:
+        _fail(f"dy must be {want} of {x.dtype}, got {tuple(dy.shape)} of {dy.dtype}")
+    dtype = dtype or weight.dtype
+    if dtype not in (weight.dtype, torch.float32):
+        _fail(f"dweight must be {weight.dtype} or torch.float32, got {dtype}")
+    _same_device(x, dy=dy)
+    dy = _pieces(dy)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if inputs else None
+    dw = torch.empty(weight.shape, dtype=dtype, device=x.device) if weights else None
+    args = [*head, 0, dy.data_ptr(), dy.stride(0), _ptr(dx), _ptr(dw), _FLOATS[dtype], 0, 0]
+    L = lm_lib()
+    ws = _workspace(_size(L.stq_expert_product_workspace, _PRODUCT.pack(*args)), x.device)
+    if ws is not None:
+        args[-2:] = ws.data_ptr(), ws.numel()
+    _call(x.device, L.stq_expert_product_backward, _PRODUCT.pack(*args))
+    return dx, dw
+
+
+class _ExpertProduct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, rows, places, offsets, gather):
+        ctx.save_for_backward(x, weight, rows, places, offsets)
+        ctx.gather = gather
+        return expert_product_forward(x, weight, ExpertPlan(rows, places, offsets), gather=gather)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, *plan = ctx.saved_tensors
+        dx, dw = expert_product_backward(dy, x, weight, ExpertPlan(*plan), gather=ctx.gather, inputs=ctx.needs_input_grad[0],
+                                         weights=ctx.needs_input_grad[1])
+        return dx, dw, None, None, None, None
+
+
+def expert_product(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *, gather: bool = False) -> torch.Tensor:
+    """``y`` of :func:`expert_product_forward`, differentiable in ``x`` and ``weight``."""
+    return _ExpertProduct.apply(x, weight, *plan, gather)
+
+
+def _combine_args(y, weights, plan):
+    yc = _float_code("y", y)
+    _check_plan(plan, y)
+    slots, shape = plan.rows.numel(), plan.places.shape
+    if y.dim() != 2 or y.shape[0] != slots:
+        _fail(f"y must be [{slots}, dim], got {tuple(y.shape)}")
+    if weights is not None and (weights.shape != shape or weights.dtype != torch.float32):
+        _fail(f"weights must be {tuple(shape)} of torch.float32, got {tuple(weights.shape)} of {weights.dtype}")
+    _same_device(y, weights=weights)
+    yr, w = _rows(y, y.shape[1]), None if weights is None else weights.contiguous()
+    n = slots // shape[-1] if shape[-1] else 0
+    head = (n, shape[-1], plan.offsets.numel() - 1, y.shape[1], yc, yr.data_ptr(), yr.stride(0), _ptr(w), plan.places.data_ptr(), plan.offsets.data_ptr())
+    return (yr, w), head
+
+
+def expert_combine_forward(y: torch.Tensor, weights: Optional[torch.Tensor], plan: ExpertPlan) -> torch.Tensor:
+    """``out`` [..., dim]: for each token the sum of ``weights`` [..., k] (fp32; None: ones) times its rows of ``y``
+    [slots, dim], added in fp32 and rounded once.  Slots of no expert add nothing."""
+    keep, head = _combine_args(y, weights, plan)
+    out = torch.empty((*plan.places.shape[:-1], y.shape[1]), dtype=y.dtype, device=y.device)
+    _call(y.device, lm_lib().stq_expert_combine_forward, _COMBINE.pack(*head, out.data_ptr(), *(0,) * 4))
+    return out
+
+
+def expert_combine_backward(dout: torch.Tensor, y: torch.Tensor, weights: Optional[torch.Tensor], plan: ExpertPlan, *,
+                            weight_grads: bool = True):
+    """``(dy, dweights)``: the gradients of ``y`` (zero in rows of no expert) and of ``weights`` (None where there are none
+    or ``weight_grads`` is False)."""
+    keep, head = _combine_args(y, weights, plan)
+    want = (*plan.places.shape[:-1], y.shape[1])
+    if dout.shape != want or dout.dtype != y.dtype:
+        _fail(f"dout must be {want} of {y.dtype}, got {tuple(dout.shape)} of {dout.dtype}")
+    _same_device(y, dout=dout)
+    g = _rows(dout, y.shape[1])
+    dy = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    dw = torch.empty(weights.shape, dtype=torch.float32, device=y.device) if weights is not None and weight_grads else None
+    _call(y.device, lm_lib().stq_expert_combine_backward, _COMBINE.pack(*head, 0, g.data_ptr(), g.stride(0), dy.data_ptr(), _ptr(dw)))
+    return dy, dw
+
+
+class _ExpertCombine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, rows, places, offsets):
+        ctx.save_for_backward(y, weights, rows, places, offsets)
+        return expert_combine_forward(y, weights, ExpertPlan(rows, places, offsets))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        y, weights, *plan = ctx.saved_tensors
+        dy, dw = expert_combine_backward(dout, y, weights, ExpertPlan(*plan), weight_grads=ctx.needs_input_grad[1])
+        return dy, dw, None, None, None
+
+
+def expert_combine(y: torch.Tensor, weights: Optional[torch.Tensor], plan: ExpertPlan) -> torch.Tensor:
+    """``out`` of :func:`expert_combine_forward`, differentiable in ``y`` and ``weights``."""
+    return _ExpertCombine.apply(y, weights, *plan)
+
+
+# ---------------------------------------------------------------- gradient clipping
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill a run of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _grad_list(grads, out):
+    """The tensors, the packed stq_grad list, and their device (None: an empty list)."""
+    grads = list(grads)
+    into = grads if out is None else list(out)
+    if len(into) != len(grads):
+        _fail(f"out must be {len(grads)} tensors, got {len(into)}")
+    flat = []
+    index = grads[0].get_device() if grads else -1
+    if grads and index < 0:
+        _fail("tensors must be CUDA")
+    for g, o in zip(grads, into):
+        code = _FLOATS.get(g.dtype)
+        if code is None:
+            _fail(f"gradients must be float32, bfloat16 or float16, got {g.dtype}")
+        if g.get_device() != index:
+            _fail(f"gradients must be on {grads[0].device}, got {g.device}")
+        if not _dense(g):
+            _fail(f"gradients must be dense, got strides {g.stride()} for {tuple(g.shape)}")
+        if o is not g and (o.dtype != g.dtype or o.shape != g.shape or o.get_device() != index or (o.stride() != g.stride() and g.numel() > 1)):
+            _fail(f"out must be like its gradient, {tuple(g.shape)} of {g.dtype} on {g.device} with the same strides")
+        flat += (g.data_ptr(), o.data_ptr(), g.numel(), code)
+    return grads, into, struct.pack(f"@{len(flat)}Q", *flat)
+
+
+def _clip(fn, grads, packed, max_norm, given):
+    dev = grads[0].device
+    norm = torch.empty((), dtype=torch.float32, device=dev) if given is None else given
+    L = lm_lib()
+    # (the list's bytes: read before the call returns)
+    buf = ctypes.create_string_buffer(packed, max(len(packed), 1))
+    args = [ctypes.addressof(buf), len(grads), max_norm, _ptr(given), norm.data_ptr(), 0, 0]
+    if given is None:
+        ws = _workspace(_size(L.stq_clip_workspace, _CLIP.pack(*args)), dev)
+        args[-2:] = ws.data_ptr(), ws.numel()
+    _call(dev, fn, _CLIP.pack(*args))
+    return norm
+
+
+def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
+    """The 2-norm of all tensors together, a fp32 scalar on their device (squares added in 64 bits)."""
+    grads, _, packed = _grad_list(grads, None)
+    if not grads:
+        _fail("no gradients")
+    return _clip(lm_lib().stq_grad_norm, grads, packed, 0.0, None)
+
+
+def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, norm: Optional[torch.Tensor] = None,
+               out: Optional[Iterable[torch.Tensor]] = None) -> torch.Tensor:
+    """Scales the gradients in place by ``min(1, max_norm / (norm + 1e-6))`` and returns their :func:`grad_norm`, without
+    a synchronisation.
+
+    ``grads``: dense fp32, bf16 or fp16 tensors of one device, apart from each other in memory.  ``out``: tensors like
+    them that take the result in their place.  ``norm``: a fp32 scalar to scale by, e.g. one formed over several ranks.
+    A norm of NaN makes every gradient NaN, an infinite one 0 (its infinite ones NaN)."""
+    grads, into, packed = _grad_list(grads, out)
+    if not grads:
+        _fail("no gradients")
+    if norm is not None:
+        if norm.numel() != 1 or norm.dtype != torch.float32:
+            _fail(f"norm must be one float32, got {tuple(norm.shape)} of {norm.dtype}")
+        _same_device(grads[0], norm=norm)
+    norm = _clip(lm_lib().stq_clip_grads, grads, packed, float(max_norm), norm)
+    _written(*into)
+    return norm
