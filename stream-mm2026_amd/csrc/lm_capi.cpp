@@ -438,6 +438,7 @@ lm::ProductArgs product_args(const stq_expert_product *a)
     o.in = (int)a->in;
     o.out = (int)a->out;
     o.k = (int)a->k;
+    o.k_inverse = a->k ? 0xffffffffu / (uint32_t)a->k : 0;
     o.tokens = a->tokens;
     o.x = a->x;
     o.x_stride = a->x_stride;

@@ -62,6 +62,7 @@ struct ProductArgs {
     int64_t slots;
     int experts, in, out;
     int k;                               // > 0: row r is token rows[r] / k of x (and of dx), 0: row r of x
+    uint32_t k_inverse;                  // (2^32 - 1) / k
     int64_t tokens;                      // k > 0: rows of x
     const void *x;
     int64_t x_stride;

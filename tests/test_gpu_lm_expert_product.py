@@ -45,11 +45,51 @@ def test_against_64_bits(n, experts, k, din, dout, dtype, gather):
     check(ids, x, w, dy, gather)
 
 
+# more tiles than workgroups, of both sizes, with tails of rows, columns and k; many rows an expert, one or none of them
+LARGE = [(4000, 4, 2, 1032, 4104), (3001, 2, 1, 72, 3080), (2500, 60, 4, 136, 4104), (9000, 1, 1, 520, 264), (700, 64, 1, 96, 2056), (513, 1, 1, 64, 64),
+         (4100, 8, 1, 128, 192)]
+
+
+@pytest.mark.parametrize("n,experts,k,din,dout", LARGE)
+@pytest.mark.parametrize("dtype,gather,skew", [(BF16, True, False), (BF16, False, True), (F16, True, True), (F16, False, False)])
+def test_many_tiles(n, experts, k, din, dout, dtype, gather, skew):
+    ids, x, w, dy = operands(n, experts, k, din, dout, dtype, gather, skew=skew, absent=0.1 if skew else 0.0)
+    check(ids, x, w, dy, gather)
+
+
+def test_one_expert_takes_all():
+    """Every other expert's run is empty; the one that is not lies first, last or between."""
+    for n in (20, 1500, 9000):
+        for e in (0, 5, 15):
+            ids, x, w, dy = operands(n, 16, 1, 80, 136, BF16, True)
+            ids.fill_(e)
+            y, dx, dw = check(ids, x, w, dy, True)
+            assert not bool(dw[[i for i in range(16) if i != e]].any())
+
+
+@pytest.mark.parametrize("experts", [63, 64, 65, 130, 512])
+def test_many_experts(experts):
+    """The search for a tile goes 64 experts at a time."""
+    for n in (experts // 3, 40 * experts):
+        ids, x, w, dy = operands(n, experts, 1, 24, 40, BF16, False, absent=0.1)
+        check(ids, x, w, dy, False)
+
+
+@pytest.mark.parametrize("n,experts,din,dout", [(30, 8, 136, 200), (900, 6, 136, 520), (5000, 4, 264, 520)])
+def test_the_same_call_gives_the_same_bits(n, experts, din, dout):
+    ids, x, w, dy = operands(n, experts, 2, din, dout, BF16, True)
+    plan = lm.expert_plan(ids, experts)
+    run = lambda: (lm.expert_product_forward(x, w, plan, gather=True), *lm.expert_product_backward(dy, x, w, plan, gather=True))  # noqa: E731
+    first = run()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, run()))
+
+
 @pytest.mark.parametrize("gather", [False, True])
 @pytest.mark.parametrize("skew", [False, True])
 def test_slots_of_no_expert(gather, skew):
     """Their rows come out as zeros and add nothing, whatever they hold."""
-    for n, experts in ((60, 20), (900, 7)):
+    for n, experts in ((60, 20), (900, 7), (2100, 2)):
         ids, x, w, dy = operands(n, experts, 2, 88, 160, BF16, gather, absent=0.3, skew=skew)
         live = int(lm.expert_plan(ids, experts).offsets[-1])
         dy[live:] = float("nan")
