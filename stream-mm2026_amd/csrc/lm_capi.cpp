@@ -512,7 +512,7 @@ int check_clip_list(const stq_clip *a)
     for (int64_t i = 0; i < a->count; i++) {
         const stq_grad &g = a->grads[i];
         if (!is_float(g.dtype)) return bad_type("gradients", g.dtype, FLOATS);
-        CHECK(check_size("elements of a gradient", g.numel, 0, (int64_t)1 << 40));
+        CHECK(check_size("elements of a gradient", g.numel, 0, lm::CLIP_MAX_NUMEL));
         if (g.numel) CHECK(check_ptr("grad", g.grad, size_of(g.dtype)));
     }
     return STQ_OK;
@@ -768,11 +768,9 @@ int stq_expert_combine_backward(const stq_expert_combine *a, void *stream)
 
 int64_t stq_clip_workspace(const stq_clip *a)
 {
-    return guarded([&]() -> int64_t {
-        if (check_clip_list(a) != STQ_OK) return -1;
-        const auto t = clip_tensors(a);
-        return lm::clip_workspace(t.data(), (int64_t)t.size());
-    }, -1);
+    if (!a) return bad("null arguments"), -1;
+    if (check_size("count", a->count, 0, 1 << 24) != STQ_OK) return -1;
+    return lm::clip_workspace(a->count);
 }
 
 int stq_grad_norm(const stq_clip *a, void *stream)
@@ -781,7 +779,7 @@ int stq_grad_norm(const stq_clip *a, void *stream)
         CHECK(check_clip_list(a));
         CHECK(check_ptr("norm", a->norm, 4));
         const auto t = clip_tensors(a);
-        CHECK(check_workspace(a->workspace, a->workspace_bytes, lm::clip_workspace(t.data(), (int64_t)t.size())));
+        CHECK(check_workspace(a->workspace, a->workspace_bytes, lm::clip_workspace(a->count)));
         return done(lm::clip_norm(t.data(), (int64_t)t.size(), (double *)a->workspace, a->norm, (hipStream_t)stream), "gradient norm");
     }, STQ_ERR_INVALID);
 }
@@ -796,7 +794,7 @@ int stq_clip_grads(const stq_clip *a, void *stream)
         if (a->given) CHECK(check_ptr("given norm", a->given, 4));
         else {
             CHECK(check_ptr("norm", a->norm, 4));
-            CHECK(check_workspace(a->workspace, a->workspace_bytes, lm::clip_workspace(t.data(), (int64_t)t.size())));
+            CHECK(check_workspace(a->workspace, a->workspace_bytes, lm::clip_workspace(a->count)));
         }
         return done(lm::clip_scale(t.data(), (int64_t)t.size(), a->max_norm, a->given, (double *)a->workspace, a->given ? nullptr : a->norm, (hipStream_t)stream),
                     "gradient clipping");

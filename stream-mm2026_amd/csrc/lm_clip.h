@@ -12,8 +12,10 @@ struct ClipTensor {
     int dt;
 };
 
-// The workspace: a double for each workgroup that adds squares.
-int64_t clip_workspace(const ClipTensor *t, int64_t count);
+// Elements of a tensor at most.
+constexpr int64_t CLIP_MAX_NUMEL = (int64_t)1 << 36;
+// The workspace in bytes: a double for each workgroup that adds squares.
+int64_t clip_workspace(int64_t count);
 // norm = sqrt(sum of all squares) into *norm (a float on the device); workspace as above.
 hipError_t clip_norm(const ClipTensor *t, int64_t count, double *partial, float *norm, hipStream_t stream);
 // out = grad min(1, max_norm / (norm + 1e-6)), the norm computed and written, or where `given` read from there.

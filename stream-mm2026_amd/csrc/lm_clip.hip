@@ -3,7 +3,7 @@
 //   norm = sqrt(sum over all tensors of g^2),  out = g min(1, max_norm / (norm + 1e-6))
 //
 // Squares and sums are doubles: no gradient that is a float overflows or vanishes in them, and the order of the sums does not
-// show in a float.  A tensor list travels as kernel arguments, 128 tensors a launch (no table to upload, so a call can
+// show in a float.  A tensor list travels as kernel arguments, 160 tensors a launch (no table to upload, so a call can
 // be captured).  Memory bound: the gradients are read twice, as their norm must be known before the first is written.
 #include "lm_clip.h"
 #include "lm_common.h"
@@ -11,31 +11,60 @@
 namespace lm {
 namespace {
 
-constexpr int LIST = 128;                 // tensors of a launch: 3.6 KB of arguments
-constexpr int TILE = 16384;               // elements a workgroup takes at a time, of one tensor
+constexpr int LIST = 160;                 // tensors of a launch: 3.8 KB of arguments
+constexpr int TILE = 32768;               // bytes a workgroup takes at a time, of one tensor (64 KB: the same times)
 constexpr int WGS = 2048;                 // workgroups of a launch at most: eight a CU, all resident
 
 struct List {
     const void *grad[LIST];
     void *out[LIST];
-    int64_t numel_dt[LIST];               // elements, and the type in the lowest two bits
-    uint32_t first[LIST];                 // its first tile
+    int64_t numel_dt[LIST];               // elements (> 0), and the type in the lowest two bits
     uint32_t tiles;                       // all tiles of the launch
     int count;
 };
 static_assert(sizeof(List) <= 4000, "kernel arguments");
 
-// Which tensor tile i belongs to: the last one that begins at or before it (tensors without tiles share their successor's
-// first).
+__host__ __device__ __forceinline__ int tile_of(int dt) { return dt == DT_F32 ? TILE / 4 : TILE / 2; }
+__host__ __device__ __forceinline__ uint32_t tiles_of(int64_t numel_dt)
+{
+    const int tile = tile_of((int)(numel_dt & 3));
+    return (uint32_t)(((numel_dt >> 2) + tile - 1) / tile);
+}
+
+// Which tensor a tile belongs to: lane l knows the first tiles of tensors l, 64 + l and 128 + l.
 struct Starts {
-    uint32_t lo, hi;
+    static constexpr int PARTS = (LIST + 63) / 64;
+    uint32_t first[PARTS];
     __device__ __forceinline__ explicit Starts(const List &l)
     {
         const int lane = threadIdx.x & 63;
-        lo = lane < l.count ? l.first[lane] : 0xffffffffu;
-        hi = 64 + lane < l.count ? l.first[64 + lane] : 0xffffffffu;
+        uint32_t before = 0;
+#pragma unroll
+        for (int p = 0; p < PARTS; p++) {
+            const int t = 64 * p + lane;
+            const uint32_t mine = t < l.count ? tiles_of(l.numel_dt[t]) : 0;
+            uint32_t upto = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t o = __shfl_up(upto, d, 64);
+                if (lane >= d) upto += o;
+            }
+            first[p] = t < l.count ? before + upto - mine : 0xffffffffu;
+            before += __builtin_amdgcn_readlane(upto, 63);
+        }
     }
-    __device__ __forceinline__ int of(uint32_t tile) const { return __popcll(__ballot(lo <= tile)) + __popcll(__ballot(hi <= tile)) - 1; }
+    // the tensor, and the tile's place in it
+    __device__ __forceinline__ int of(uint32_t tile, uint32_t &in) const
+    {
+        int t = -1;
+#pragma unroll
+        for (int p = 0; p < PARTS; p++) t += __popcll(__ballot(first[p] <= tile));
+        in = tile;
+#pragma unroll
+        for (int p = 0; p < PARTS; p++)
+            if (t >> 6 == p) in -= __builtin_amdgcn_readlane(first[p], t & 63);
+        return t;
+    }
 };
 
 __device__ __forceinline__ double wave_add(double v)
@@ -89,9 +118,11 @@ __global__ __launch_bounds__(256) void clip_norm_kernel(List l, double *partial)
     const Starts starts(l);
     double s = 0.0;
     for (uint32_t tile = blockIdx.x; tile < l.tiles; tile += gridDim.x) {
-        const int t = starts.of(tile);
-        const int64_t numel = l.numel_dt[t] >> 2, at = (int64_t)(tile - l.first[t]) * TILE;
-        const int n = (int)(numel - at < TILE ? numel - at : TILE), dt = (int)(l.numel_dt[t] & 3);
+        uint32_t in;
+        const int t = starts.of(tile, in);
+        const int dt = (int)(l.numel_dt[t] & 3), tile_n = tile_of(dt);
+        const int64_t numel = l.numel_dt[t] >> 2, at = (int64_t)in * tile_n;
+        const int n = (int)(numel - at < tile_n ? numel - at : tile_n);
         if (dt == DT_F32) s += squares<DT_F32>(l.grad[t], at, n);
         else if (dt == DT_BF16) s += squares<DT_BF16>(l.grad[t], at, n);
         else s += squares<DT_F16>(l.grad[t], at, n);
@@ -165,11 +196,13 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(List l, const double *p
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
     for (uint32_t i = blockIdx.x; i < l.tiles; i += gridDim.x) {
         const uint32_t tile = l.tiles - 1 - i;
-        const int t = starts.of(tile);
+        uint32_t in;
+        const int t = starts.of(tile, in);
         // gradients in place that keep their values need no write
         if (c.one() && l.grad[t] == l.out[t]) continue;
-        const int64_t numel = l.numel_dt[t] >> 2, at = (int64_t)(tile - l.first[t]) * TILE;
-        const int n = (int)(numel - at < TILE ? numel - at : TILE), dt = (int)(l.numel_dt[t] & 3);
+        const int dt = (int)(l.numel_dt[t] & 3), tile_n = tile_of(dt);
+        const int64_t numel = l.numel_dt[t] >> 2, at = (int64_t)in * tile_n;
+        const int n = (int)(numel - at < tile_n ? numel - at : tile_n);
         if (dt == DT_F32) scale_tile<DT_F32>(l.grad[t], l.out[t], at, n, c);
         else if (dt == DT_BF16) scale_tile<DT_BF16>(l.grad[t], l.out[t], at, n, c);
         else scale_tile<DT_F16>(l.grad[t], l.out[t], at, n, c);
@@ -179,20 +212,17 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(List l, const double *p
 // Tensors from `i` on as one launch's list; where the next begins.
 int64_t gather(const ClipTensor *t, int64_t count, int64_t i, List &l)
 {
-    uint64_t tiles = 0;
+    uint32_t tiles = 0;                   // (below 2^31: CLIP_MAX_NUMEL)
     l.count = 0;
     for (; i < count && l.count < LIST; i++) {
         if (t[i].numel == 0) continue;
-        const uint64_t mine = (t[i].numel + TILE - 1) / TILE;
-        if (tiles + mine > 0xfffffff0ull) break;
         const int k = l.count++;
         l.grad[k] = t[i].grad;
         l.out[k] = t[i].out;
         l.numel_dt[k] = t[i].numel << 2 | t[i].dt;
-        l.first[k] = (uint32_t)tiles;
-        tiles += mine;
+        tiles += tiles_of(l.numel_dt[k]);
     }
-    l.tiles = (uint32_t)tiles;
+    l.tiles = tiles;
     return i;
 }
 unsigned wgs_of(const List &l) { return l.tiles < WGS ? l.tiles : WGS; }
@@ -214,16 +244,9 @@ hipError_t norm_launches(const ClipTensor *t, int64_t count, double *partial, in
 
 }  // namespace
 
-int64_t clip_workspace(const ClipTensor *t, int64_t count)
-{
-    int64_t partials = 1;
-    List l;
-    for (int64_t i = 0; i < count;) {
-        i = gather(t, count, i, l);
-        partials += wgs_of(l);
-    }
-    return partials * 8;
-}
+static_assert((CLIP_MAX_NUMEL * 4 / TILE) * LIST < (1ll << 31), "tiles of a launch");
+
+int64_t clip_workspace(int64_t count) { return ((count + LIST - 1) / LIST * WGS + 1) * 8; }
 
 hipError_t clip_norm(const ClipTensor *t, int64_t count, double *partial, float *norm, hipStream_t stream)
 {

@@ -223,7 +223,7 @@ __device__ __forceinline__ void wait_loads()
 
 // GATHER: row r is token rows[r] / k of x; DX: the result goes to scratch, in fp32.
 template <int DT, int FORM, bool GATHER, int BM, int BN, int WM, int WN, int BK, int STAGES>
-__global__ __launch_bounds__(WM *WN * 64, BM *BN / (WM * WN) > 128 * 64 ? 1 : 2) void product_kernel(ProductArgs a, int m_tiles, int n_tiles)
+__global__ __launch_bounds__(WM *WN * 64, 2) void product_kernel(ProductArgs a, int m_tiles, int n_tiles)
 {
     constexpr int THREADS = WM * WN * 64, MI = BM / WM / 32, NI = BN / WN / 32;
     using OpA = Operand<BM, FORM != DWEIGHT, THREADS, BK>;
@@ -497,7 +497,7 @@ hipError_t launch(const ProductArgs &a, hipStream_t stream)
     int64_t tiles = FORM == DWEIGHT ? a.experts * m_tiles * n_tiles : (a.slots / BM + parts) * n_tiles;
     if (tiles == 0) return hipSuccess;
     // as many workgroups as the 256 CUs hold, an eighth of them on each XCD
-    constexpr int RESIDENT = 256 * (STAGES * (BM + BN) * BK * 2 + WM * WN * 4096 > 80 * 1024 ? 1 : 2);
+    constexpr int RESIDENT = 256 * (160 * 1024 / (STAGES * (BM + BN) * BK * 2 + WM * WN * 4096));
     tiles = (tiles + 7) / 8 * 8;
     product_kernel<DT, FORM, GATHER, BM, BN, WM, WN, BK, STAGES><<<(unsigned)(tiles < RESIDENT ? tiles : RESIDENT), WM * WN * 64, 0, stream>>>(a, (int)m_tiles, (int)n_tiles);
     return hipGetLastError();

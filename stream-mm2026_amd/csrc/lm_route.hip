@@ -13,7 +13,7 @@
 namespace lm {
 namespace {
 
-constexpr int ROUTE_WGS = 512;            // workgroups at most: each adds a row of partial loads
+constexpr int ROUTE_WGS = 1024;           // workgroups at most: each adds a row of partial loads
 
 // A float as an integer of the same order, NaN above all, -0 as 0; 0: absent (-inf, or no expert).
 __device__ __forceinline__ uint32_t ordered(float z)
@@ -29,12 +29,28 @@ __device__ __forceinline__ float from_ordered(uint32_t key)
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// Over the L lanes of a row, the same bits on each of them.
+// Over the L lanes of a row without LDS: pairs, quads, halves and rows of 16 mirrored (DPP), then rows and halves of the wave
+// swapped.  Both sides of each exchange combine the same two values, so every lane ends with the same bits.
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
 template <int L, typename T, typename F>
 __device__ __forceinline__ T row_reduce(T v, F op)
 {
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) v = op(v, __shfl_xor(v, d, 64));
+    auto with = [&](uint32_t other) { return op(v, __builtin_bit_cast(T, other)); };
+    v = with(moved<0xb1>(__builtin_bit_cast(uint32_t, v)));
+    v = with(moved<0x4e>(__builtin_bit_cast(uint32_t, v)));
+    v = with(moved<0x141>(__builtin_bit_cast(uint32_t, v)));
+    if constexpr (L >= 16) v = with(moved<0x140>(__builtin_bit_cast(uint32_t, v)));
+    if constexpr (L >= 32) {
+        const uint32_t w = __builtin_bit_cast(uint32_t, v);
+        const auto rows = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+        v = op(__builtin_bit_cast(T, (uint32_t)rows[0]), __builtin_bit_cast(T, (uint32_t)rows[1]));
+    }
+    if constexpr (L >= 64) {
+        const uint32_t w = __builtin_bit_cast(uint32_t, v);
+        const auto halves = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+        v = op(__builtin_bit_cast(T, (uint32_t)halves[0]), __builtin_bit_cast(T, (uint32_t)halves[1]));
+    }
     return v;
 }
 struct MaxKey {
@@ -47,15 +63,19 @@ struct Row {
     float z[C], p[C];
     float top, total;
 
-    __device__ __forceinline__ void read(const RouteArgs &a, int64_t row, int l, bool live)
+    __device__ __forceinline__ void read(const RouteArgs &a, int64_t row, int l)
     {
-        top = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < C; i++) {
             const int e = l + L * i;
-            z[i] = live && e < a.experts ? Elem<DT>::load(a.logits, row * a.stride + e) : -__builtin_inff();
-            top = Max()(top, z[i]);
+            z[i] = row < a.n && e < a.experts ? Elem<DT>::load(a.logits, row * a.stride + e) : -__builtin_inff();
         }
+    }
+    __device__ __forceinline__ void softmax()
+    {
+        top = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < C; i++) top = Max()(top, z[i]);
         top = row_reduce<L>(top, Max());
         const float from = top == -__builtin_inff() ? 0.0f : top;
         total = 0.0f;
@@ -78,11 +98,14 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a)
     __shared__ float sums[ROWS][L * C];
     const int lane = threadIdx.x & 63, l = threadIdx.x & (L - 1), r = threadIdx.x / L, first = lane & ~(L - 1);
     float load[C] = {};
+    Row<DT, L, C> x, next;
+    next.read(a, (int64_t)blockIdx.x * ROWS + r, l);
     for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.n; row0 += (int64_t)gridDim.x * ROWS) {
         const int64_t row = row0 + r;
         const bool live = row < a.n;
-        Row<DT, L, C> x;
-        x.read(a, row, l, live);
+        x = next;
+        next.read(a, row + (int64_t)gridDim.x * ROWS, l);
+        x.softmax();
         uint32_t key[C];
 #pragma unroll
         for (int i = 0; i < C; i++) {
@@ -90,7 +113,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a)
             load[i] += x.p[i];
         }
         // the k largest in turn; lane j of the row keeps the j-th (as many as 64 of them: a row of 64 lanes)
-        float mine = 0.0f, chosen = 0.0f;
+        uint32_t mine = 0;
         int id = -1;
         for (int j = 0; j < a.k; j++) {
             uint32_t best = 0;
@@ -109,16 +132,16 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a)
                     if (l == who) key[i] = 0;
                 }
             }
-            const float w = at < 0 ? 0.0f : expf(from_ordered(best) - x.top) / x.total;
-            chosen += w;
             if (l == j) {
-                mine = w;
+                mine = best;
                 id = at;
             }
         }
+        float w = id < 0 ? 0.0f : expf(from_ordered(mine) - x.top) / x.total;
+        const float chosen = row_reduce<L>(w, Add());
         if (live && l < a.k) {
-            if (a.renormalize && id >= 0) mine /= chosen;
-            a.weights[row * a.k + l] = mine;
+            if (a.renormalize && id >= 0) w /= chosen;
+            a.weights[row * a.k + l] = w;
             a.ids[row * a.k + l] = id;
         }
     }
@@ -162,7 +185,8 @@ __global__ __launch_bounds__(256) void route_back_kernel(RouteArgs a)
         const int64_t row = row0 + r;
         const bool live = row < a.n;
         Row<DT, L, C> x;
-        x.read(a, row, l, live);
+        x.read(a, row, l);
+        x.softmax();
         // lane j: the j-th choice
         int id = -1;
         float w = 0.0f, dw = 0.0f;
@@ -248,7 +272,15 @@ __global__ __launch_bounds__(PLAN_WAVES * 64) void plan_kernel(PlanArgs a, int64
     for (int i = threadIdx.x; i < PLAN_WAVES * (EXPERT_MAX + 1); i += PLAN_WAVES * 64) (&count[0][0])[i] = 0;
     __syncthreads();
     const int64_t first = min(a.slots, ((int64_t)blockIdx.x * PLAN_WAVES + wave) * each), last = min(a.slots, first + each);
-    for (int64_t i = first + lane; i < last; i += 64) atomicAdd(&count[wave][bucket(a.ids, a.id_bytes, i, a.experts)], 1);
+    // (four loads on their way at a time)
+    for (int64_t i0 = first + lane; i0 < last; i0 += 4 * 64) {
+        int e[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) e[u] = i0 + 64 * u < last ? bucket(a.ids, a.id_bytes, i0 + 64 * u, a.experts) : -1;
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (e[u] >= 0) atomicAdd(&count[wave][e[u]], 1);
+    }
     __syncthreads();
     const int b = threadIdx.x;
     int here = 0;
@@ -263,6 +295,7 @@ __global__ __launch_bounds__(PLAN_WAVES * 64) void plan_kernel(PlanArgs a, int64
     if constexpr (!ALONE) {
         total = 0;
         if (b < buckets)
+#pragma unroll 8
             for (int g = 0; g < (int)gridDim.x; g++) {
                 const int n = a.hist[(int64_t)g * buckets + b];
                 before += g < (int)blockIdx.x ? n : 0;
@@ -291,23 +324,32 @@ __global__ __launch_bounds__(PLAN_WAVES * 64) void plan_kernel(PlanArgs a, int64
     __syncthreads();
     const int bits = 32 - __builtin_clz(buckets);
     const uint64_t lower = (1ull << lane) - 1;
-    for (int64_t i0 = first; i0 < last; i0 += 64) {
-        const int64_t i = i0 + lane;
-        const bool valid = i < last;
-        const int e = valid ? bucket(a.ids, a.id_bytes, i, a.experts) : 0;
-        uint64_t same = __ballot(valid);
-        for (int k = 0; k < bits; k++) {
-            const uint64_t set = __ballot(valid && (e >> k & 1));
-            same &= e >> k & 1 ? set : ~set;
+    for (int64_t i0 = first; i0 < last; i0 += 4 * 64) {
+        int e[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int64_t i = i0 + 64 * u + lane;
+            e[u] = i < last ? bucket(a.ids, a.id_bytes, i, a.experts) : -1;
         }
-        int at = 0;
-        if (valid) at = count[wave][e] + __popcll(same & lower);
-        __builtin_amdgcn_wave_barrier();
-        if (valid && !(same & lower)) count[wave][e] += __popcll(same);
-        __builtin_amdgcn_wave_barrier();
-        if (valid) {
-            a.rows[at] = (int)i;
-            a.places[i] = at;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const bool valid = e[u] >= 0;
+            uint64_t same = __ballot(valid);
+            if (same == 0) break;
+            for (int k = 0; k < bits; k++) {
+                const uint64_t set = __ballot(valid && (e[u] >> k & 1));
+                same &= e[u] >> k & 1 ? set : ~set;
+            }
+            int at = 0;
+            if (valid) at = count[wave][e[u]] + __popcll(same & lower);
+            __builtin_amdgcn_wave_barrier();
+            if (valid && !(same & lower)) count[wave][e[u]] += __popcll(same);
+            __builtin_amdgcn_wave_barrier();
+            if (valid) {
+                const int64_t i = i0 + 64 * u + lane;
+                a.rows[at] = (int)i;
+                a.places[i] = at;
+            }
         }
     }
 }

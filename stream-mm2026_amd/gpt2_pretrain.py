@@ -37,6 +37,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 if _HERE not in sys.path:
     sys.path.insert(0, _HERE)
 
+from stquant_lm import clip_grads  # noqa: E402
 from stquant_opt_fused_io import MDQAdamWSimpleFusedIO  # noqa: E402
 from stquant_opt_simple import MDQAdamWSimple  # noqa: E402
 
@@ -117,13 +118,14 @@ def train(optimizer_name: str = "MDQAdamW-Simple-FusedIO", *, steps: int = 300, 
           batch: int = 8, seq_len: int = 1024, lr: float = 2e-4, bits=4, block_size: int = 128,
           rounding: str = "stochastic", data_seed: int = 1234, model_seed: int = 42, opt_seed: int = 0,
           n_layer: int = 12, n_embd: int = 768, n_head: int = 12, vocab_used: int = VOCAB,
-          device="cuda:0", log_every: int = 0, fused_transitions: bool = True):
+          device="cuda:0", log_every: int = 0, fused_transitions: bool = True, max_grad_norm: float = 0.0):
     """Run ``warmup`` untimed-history steps then ``steps`` measured steps; return the summary.
 
     Tokens are uniform over ``[0, vocab_used)`` (the full vocabulary by default; a smaller range
     gives a learnable unigram task whose loss falls towards ``log(vocab_used)``).  ``bits=None``
     runs the MDQ score-based bit schedule; ``fused_transitions=False`` steps tensors whose bit
-    width changes with separate conversion passes instead of the storage-changing kernel."""
+    width changes with separate conversion passes instead of the storage-changing kernel.
+    ``max_grad_norm`` > 0: the gradients are clipped to that norm, as part of the optimizer's step."""
     dev = torch.device(device)
     model = build_model(dev, n_layer=n_layer, n_embd=n_embd, n_head=n_head, n_positions=seq_len,
                         seed=model_seed)
@@ -159,6 +161,8 @@ def train(optimizer_name: str = "MDQAdamW-Simple-FusedIO", *, steps: int = 300, 
         out.loss.backward()
         sync()
         t2 = time.perf_counter()
+        if max_grad_norm > 0:
+            clip_grads([p.grad for p in model.parameters() if p.grad is not None], max_grad_norm)
         opt.step()
         sync()
         t3 = time.perf_counter()
@@ -247,10 +251,11 @@ def main(argv=None):
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--seq-len", type=int, default=1024)
     ap.add_argument("--lr", type=float, default=2e-4)
+    ap.add_argument("--max-grad-norm", type=float, default=0.0)
     ap.add_argument("--out", default=None, help="write the summary (with history) as JSON here")
     a = ap.parse_args(argv)
     res = train(a.optimizer, steps=a.steps, warmup=a.warmup, batch=a.batch, seq_len=a.seq_len, lr=a.lr,
-                bits=a.bits, block_size=a.block_size, rounding=a.rounding, log_every=25)
+                bits=a.bits, block_size=a.block_size, rounding=a.rounding, log_every=25, max_grad_norm=a.max_grad_norm)
     if a.out:
         with open(a.out, "w") as f:
             json.dump(res, f, indent=1)

@@ -24,6 +24,7 @@ tensors' type, and the same call gives the same bits every time.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 import sys
@@ -561,6 +562,22 @@ def distill_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids
 
 
 # ---------------------------------------------------------------- routing to experts
+# (sizes follow from sizes: asked for once)
+@functools.lru_cache(maxsize=1024)
+def _route_workspace(n: int, experts: int, k: int, code: int) -> int:
+    return _size(lm_lib().stq_route_workspace, _ROUTE.pack(n, experts, k, code, *(0,) * 12))
+
+
+@functools.lru_cache(maxsize=1024)
+def _plan_workspace(slots: int, experts: int) -> int:
+    return _size(lm_lib().stq_expert_plan_workspace, _PLAN.pack(0, 7, slots, experts, *(0,) * 5))
+
+
+@functools.lru_cache(maxsize=1024)
+def _clip_workspace(count: int) -> int:
+    return _size(lm_lib().stq_clip_workspace, _CLIP.pack(0, count, 0.0, *(0,) * 4))
+
+
 def _route_args(logits, k):
     """The checked logits as rows, and the struct's leading fields but for renormalize."""
     zc = _float_code("logits", logits)
@@ -584,11 +601,10 @@ def route_forward(logits: torch.Tensor, k: int, *, renormalize: bool = False):
     weights = torch.empty((*lead, head[2]), dtype=torch.float32, device=z.device)
     ids = torch.empty((*lead, head[2]), dtype=torch.int32, device=z.device)
     load = torch.empty((head[1],), dtype=torch.float32, device=z.device)
-    args = [*head, int(renormalize), z.data_ptr(), z.stride(0), weights.data_ptr(), ids.data_ptr(), load.data_ptr(), *(0,) * 6]
-    L = lm_lib()
-    ws = _workspace(_size(L.stq_route_workspace, _ROUTE.pack(*args)), z.device)
-    args[-2:] = ws.data_ptr(), ws.numel()
-    _call(z.device, L.stq_route_forward, _ROUTE.pack(*args))
+    ws = _workspace(_route_workspace(*head), z.device)
+    _call(z.device, lm_lib().stq_route_forward,
+          _ROUTE.pack(*head, int(renormalize), z.data_ptr(), z.stride(0), weights.data_ptr(), ids.data_ptr(), load.data_ptr(), 0, 0, 0, 0,
+                      ws.data_ptr(), ws.numel()))
     return weights, ids, load
 
 
@@ -655,12 +671,9 @@ def expert_plan(ids: torch.Tensor, experts: int) -> ExpertPlan:
     rows = torch.empty((n,), dtype=torch.int32, device=ids.device)
     places = torch.empty(ids.shape, dtype=torch.int32, device=ids.device)
     offsets = torch.empty((max(int(experts), 0) + 1,), dtype=torch.int32, device=ids.device)
-    args = [ids.data_ptr(), ic, n, int(experts), rows.data_ptr(), places.data_ptr(), offsets.data_ptr(), 0, 0]
-    L = lm_lib()
-    ws = _workspace(_size(L.stq_expert_plan_workspace, _PLAN.pack(*args)), ids.device)
-    if ws is not None:
-        args[-2:] = ws.data_ptr(), ws.numel()
-    _call(ids.device, L.stq_expert_plan_sort, _PLAN.pack(*args))
+    ws = _workspace(_plan_workspace(n, int(experts)), ids.device)
+    _call(ids.device, lm_lib().stq_expert_plan_sort,
+          _PLAN.pack(ids.data_ptr(), ic, n, int(experts), rows.data_ptr(), places.data_ptr(), offsets.data_ptr(), _ptr(ws), 0 if ws is None else ws.numel()))
     return ExpertPlan(rows, places, offsets)
 
 
@@ -858,14 +871,10 @@ def _grad_list(grads, out):
 def _clip(fn, grads, packed, max_norm, given):
     dev = grads[0].device
     norm = torch.empty((), dtype=torch.float32, device=dev) if given is None else given
-    L = lm_lib()
     # (the list's bytes: read before the call returns)
-    buf = ctypes.create_string_buffer(packed, max(len(packed), 1))
-    args = [ctypes.addressof(buf), len(grads), max_norm, _ptr(given), norm.data_ptr(), 0, 0]
-    if given is None:
-        ws = _workspace(_size(L.stq_clip_workspace, _CLIP.pack(*args)), dev)
-        args[-2:] = ws.data_ptr(), ws.numel()
-    _call(dev, fn, _CLIP.pack(*args))
+    buf = ctypes.create_string_buffer(packed, len(packed))
+    ws = _workspace(_clip_workspace(len(grads)), dev)
+    _call(dev, fn, _CLIP.pack(ctypes.addressof(buf), len(grads), max_norm, _ptr(given), norm.data_ptr(), ws.data_ptr(), ws.numel()))
     return norm
 
 

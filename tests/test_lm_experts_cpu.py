@@ -45,7 +45,7 @@ def route(backward=False, **kw):
     (False, dict(ids=P + 1), "ids must be aligned to 4 bytes"),
     (False, dict(load=P + 1), "load must be aligned to 4 bytes"),
     (False, dict(ws=0), "workspace: null data pointer"),
-    (False, dict(wsn=100), "workspace needs 16384 bytes, got 100"),
+    (False, dict(wsn=100), "workspace needs 32768 bytes, got 100"),
     (True, dict(dz=0), "dlogits: null data pointer"),
     (True, dict(dzs=7), "rows of dlogits must not overlap"),
     (True, dict(dw=P + 2), "dweights must be aligned to 4 bytes"),
@@ -169,7 +169,7 @@ OVERLAP = "gradients that are written must not overlap others"
     ([(A, A, 10, 0)], dict(max_norm=float("nan")), "max_norm must be >= 0"),
     ([(A, A, 10, 0)], dict(norm=0), "norm: null data pointer"),
     ([(A, A, 10, 0)], dict(given=P + 2), "given norm must be aligned to 4 bytes"),
-    ([(A, A, 10, 0)], dict(wsn=8), "workspace needs 16 bytes, got 8"),
+    ([(A, A, 10, 0)], dict(wsn=8), "workspace needs 16392 bytes, got 8"),
     ([(A, A, 10, 0)], dict(ws=P + 8), "workspace must be aligned to 16 bytes"),
     ([(A, A, 10, 0)], dict(null=True), "grads: null data pointer"),
     ([(A, A, 10, 0)], dict(count=-1), "count must be 0 to"),
