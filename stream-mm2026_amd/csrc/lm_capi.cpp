@@ -526,7 +526,7 @@ int check_clip_apart(const stq_clip *a)
         int64_t of;                       // the tensor; < 0: written, ~tensor
     };
     std::vector<Span> spans;
-    spans.reserve(2 * a->count);
+    spans.reserve(2 * a->count + 1);
     for (int64_t i = 0; i < a->count; i++) {
         const stq_grad &g = a->grads[i];
         if (g.numel == 0) continue;
@@ -535,11 +535,12 @@ int check_clip_apart(const stq_clip *a)
         spans.push_back({(const char *)g.out, (const char *)g.out + bytes, ~i});
         if (g.out != g.grad) spans.push_back({(const char *)g.grad, (const char *)g.grad + bytes, i});
     }
+    if (a->given) spans.push_back({(const char *)a->given, (const char *)(a->given + 1), a->count});
     std::sort(spans.begin(), spans.end(), [](const Span &x, const Span &y) { return x.from < y.from; });
     // the farthest ends so far, of all spans and of those written
     const char *any = nullptr, *written = nullptr;
     for (const Span &s : spans) {
-        if ((s.of < 0 && any > s.from) || written > s.from) return bad("gradients that are written must not overlap others");
+        if ((s.of < 0 && any > s.from) || written > s.from) return bad("gradients that are written must not overlap others, or the given norm");
         any = std::max(any, s.to);
         if (s.of < 0) written = std::max(written, s.to);
     }

@@ -531,48 +531,48 @@ __global__ __launch_bounds__(256) void product_few_kernel(ProductArgs a, int n_t
     tiles.m_tiles = 0;
     tiles.n_tiles = n_tiles;
     tiles.of_rows(a.offsets, FEW_M);
-    Tile t;
-    if (!tiles.next_of_rows(a.offsets, FEW_M, t)) return;
-    const int m = t.m * FEW_M + (lane & 15), n0 = t.n * FEW_N, piece = (lane >> 4) * 8;
-    const bool here = t.first + m < t.last;
-    f32x4 acc[2] = {};
-    if (t.expert < a.experts) {
-        const char *const x = (const char *)a.x + (here ? source_row<GATHER>(a, t.first + m) * a.x_stride + piece : 0) * 2;
-        const char *w[2];
+    for (Tile t; tiles.next_of_rows(a.offsets, FEW_M, t); __syncthreads()) {
+        const int m = t.m * FEW_M + (lane & 15), n0 = t.n * FEW_N, piece = (lane >> 4) * 8;
+        const bool here = t.first + m < t.last;
+        f32x4 acc[2] = {};
+        if (t.expert < a.experts) {
+            const char *const x = (const char *)a.x + (here ? source_row<GATHER>(a, t.first + m) * a.x_stride + piece : 0) * 2;
+            const char *w[2];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-            w[i] = (const char *)a.weight + ((int64_t)t.expert * a.weight_expert_stride + min(n0 + 16 * i + (lane & 15), a.out - 1) * a.weight_row_stride + piece) * 2;
-        for (int k0 = wave * 64; k0 < a.in; k0 += 256 * FLY) {
-            u32x4 fx[FLY][2], fw[FLY][2][2];
+            for (int i = 0; i < 2; i++)
+                w[i] = (const char *)a.weight + ((int64_t)t.expert * a.weight_expert_stride + min(n0 + 16 * i + (lane & 15), a.out - 1) * a.weight_row_stride + piece) * 2;
+            for (int k0 = wave * 64; k0 < a.in; k0 += 256 * FLY) {
+                u32x4 fx[FLY][2], fw[FLY][2][2];
 #pragma unroll
-            for (int u = 0; u < FLY; u++)
+                for (int u = 0; u < FLY; u++)
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const int k = k0 + 256 * u + 32 * s;
-                    const bool in = k + piece < a.in;
+                    for (int s = 0; s < 2; s++) {
+                        const int k = k0 + 256 * u + 32 * s;
+                        const bool in = k + piece < a.in;
 #pragma unroll
-                    for (int i = 0; i < 2; i++) fw[u][s][i] = in ? *(const u32x4 *)(w[i] + k * 2) : u32x4{};
-                    fx[u][s] = in && here ? *(const u32x4 *)(x + k * 2) : u32x4{};
-                }
+                        for (int i = 0; i < 2; i++) fw[u][s][i] = in ? *(const u32x4 *)(w[i] + k * 2) : u32x4{};
+                        fx[u][s] = in && here ? *(const u32x4 *)(x + k * 2) : u32x4{};
+                    }
 #pragma unroll
-            for (int u = 0; u < FLY; u++)
+                for (int u = 0; u < FLY; u++)
 #pragma unroll
-                for (int s = 0; s < 2; s++)
+                    for (int s = 0; s < 2; s++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++) acc[i] = mma16<DT>(fw[u][s][i], fx[u][s], acc[i]);
+                        for (int i = 0; i < 2; i++) acc[i] = mma16<DT>(fw[u][s][i], fx[u][s], acc[i]);
+            }
         }
-    }
-    if (wave)
+        if (wave)
 #pragma unroll
-        for (int i = 0; i < 2; i++) sums[wave - 1][i][lane] = acc[i];
-    __syncthreads();
-    if (wave || !here) return;
+            for (int i = 0; i < 2; i++) sums[wave - 1][i][lane] = acc[i];
+        __syncthreads();
+        if (wave || !here) continue;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const f32x4 v = ((acc[i] + sums[0][i][lane]) + sums[1][i][lane]) + sums[2][i][lane];
-        const int n = n0 + 16 * i + 4 * (lane >> 4);
-        const float f[4] = {v[0], v[1], v[2], v[3]};
-        if (n < a.out) store_n<DT, 4>(a.y, (int64_t)(t.first + m) * a.out + n, f);
+        for (int i = 0; i < 2; i++) {
+            const f32x4 v = ((acc[i] + sums[0][i][lane]) + sums[1][i][lane]) + sums[2][i][lane];
+            const int n = n0 + 16 * i + 4 * (lane >> 4);
+            const float f[4] = {v[0], v[1], v[2], v[3]};
+            if (n < a.out) store_n<DT, 4>(a.y, (int64_t)(t.first + m) * a.out + n, f);
+        }
     }
 }
 
@@ -580,8 +580,9 @@ template <int DT, bool GATHER>
 hipError_t launch_few(const ProductArgs &a, hipStream_t stream)
 {
     const int64_t n_tiles = (a.out + FEW_N - 1) / FEW_N, parts = a.slots < a.experts + 1 ? a.slots : a.experts + 1;
+    constexpr int64_t MOST = 1 << 16;          // (each takes several tiles then)
     const int64_t wgs = ((a.slots / FEW_M + parts) * n_tiles + 7) / 8 * 8;
-    product_few_kernel<DT, GATHER><<<(unsigned)wgs, 256, 0, stream>>>(a, (int)n_tiles);
+    product_few_kernel<DT, GATHER><<<(unsigned)(wgs < MOST ? wgs : MOST), 256, 0, stream>>>(a, (int)n_tiles);
     return hipGetLastError();
 }
 

@@ -75,6 +75,13 @@ def test_many_experts(experts):
         check(ids, x, w, dy, False)
 
 
+def test_few_rows_and_more_tiles_than_workgroups():
+    ids, x, w, dy = operands(256, 64, 2, 8, 131080, BF16, True)
+    plan = lm.expert_plan(ids, 64)
+    y = lm.expert_product_forward(x, w, plan, gather=True)
+    er.check_product(dict(y=y), er.product(x, w, ids, True), dict(y=8))
+
+
 @pytest.mark.parametrize("n,experts,din,dout", [(30, 8, 136, 200), (900, 6, 136, 520), (5000, 4, 264, 520)])
 def test_the_same_call_gives_the_same_bits(n, experts, din, dout):
     ids, x, w, dy = operands(n, experts, 2, din, dout, BF16, True)

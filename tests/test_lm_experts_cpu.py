@@ -180,6 +180,7 @@ OVERLAP = "gradients that are written must not overlap others"
     ([(A, A + 8, 10, 0)], {}, OVERLAP),                                  # an output inside its own gradient
     ([(A, B, 10, 0), (B + 36, B + 4096, 10, 0)], {}, OVERLAP),           # an output inside another gradient
     ([(A, A, 1000, 0), (A + 8, B, 1, 0), (A + 64, B + 64, 1, 0)], {}, OVERLAP),
+    ([(A, A, 1000, 0)], dict(given=A + 400), OVERLAP),                   # a given norm inside a gradient that is written
 ])
 def test_clip_refusals(grads, kw, msg):
     assert clip(grads, **kw) == INVALID and msg in err()
