@@ -6,7 +6,9 @@
 //   dz = p (dl - <p, dl> - [not renormalised] <w, dw>) + [chosen] w (dw - [renormalised] <w, dw>)
 //
 // Rows are short (experts), so they live in registers: a row's experts are spread over 8 to 64 lanes, several rows a wave
-// where they are few.  What bounds these kernels is latency, launches above all.
+// where they are few.  What bounds these kernels is latency, launches above all: 8192 rows of 64 experts with 6 choices take 8.5
+// us for the choices (15 with exchanges through LDS and an exponential a choice), 4 for the load's sums, 13 for the plan
+// and 5.7 for the gradient, of 1 MB each way.
 #include "lm_common.h"
 #include "lm_expert.h"
 
@@ -366,8 +368,8 @@ int plan_wgs(int64_t slots)
 }
 
 // ---------------------------------------------------------------- combination
-// A wave a token: its k rows of y are read piece by piece, four of them in flight.  Bound by memory.  Pieces are taken at any
-// alignment, so that the order of a sum does not go by it.
+// A wave a token: its k rows of y are read piece by piece, four of them in flight.  Bound by memory: 16384 x 2 rows of 4096 (bf16) 90
+// us, 4.3 TB/s, and backward 139, 4.7.  Pieces are taken at any alignment, so that the order of a sum does not go by it.
 constexpr int COMBINE_WGS = 1 << 16;
 
 // N elements of a row of dim from column c on: the last piece may be short.

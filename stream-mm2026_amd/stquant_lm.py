@@ -860,9 +860,11 @@ def _grad_list(grads, out):
             _fail(f"gradients must be float32, bfloat16 or float16, got {g.dtype}")
         if g.get_device() != index:
             _fail(f"gradients must be on {grads[0].device}, got {g.device}")
-        if not _dense(g):
+        plain = g.is_contiguous()
+        if not plain and not _dense(g):
             _fail(f"gradients must be dense, got strides {g.stride()} for {tuple(g.shape)}")
-        if o is not g and (o.dtype != g.dtype or o.shape != g.shape or o.get_device() != index or (o.stride() != g.stride() and g.numel() > 1)):
+        if o is not g and (o.dtype != g.dtype or o.get_device() != index or o.shape != g.shape
+                           or not (plain and o.is_contiguous() or g.numel() < 2 or o.stride() == g.stride())):
             _fail(f"out must be like its gradient, {tuple(g.shape)} of {g.dtype} on {g.device} with the same strides")
         flat += (g.data_ptr(), o.data_ptr(), g.numel(), code)
     return grads, into, struct.pack(f"@{len(flat)}Q", *flat)
