@@ -179,7 +179,7 @@ __device__ __forceinline__ void scale_tile(const void *p, void *out, int64_t at,
             if (i + u * 256 < pieces) {
 #pragma unroll
                 for (int k = 0; k < PER; k++) v[u][k] = c.of(v[u][k]);
-                store_n<DT, PER, true>(out, at + (int64_t)(i + u * 256) * PER, v[u]);
+                __builtin_nontemporal_store(Elem<DT>::pack(v[u]), (u32x4_any *)((char *)out + (at + (int64_t)(i + u * 256) * PER) * Elem<DT>::SIZE));
             }
     }
     const int rest = pieces * PER + threadIdx.x;

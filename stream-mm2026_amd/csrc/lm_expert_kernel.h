@@ -449,7 +449,11 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void product_kernel(ProductArgs a, 
             for (int q = 0; q < 4; q++) {
                 const int row = 8 * q + store_row, m = m0 + wm + 32 * j + row, at = n + store_piece * (16 / size);
                 const u32x4 w = *(const __attribute__((address_space(3))) u32x4 *)(mine + row * 128 + ((store_piece ^ (row >> 1 & 7)) << 4));
-                if (m < M && at < N) *(u32x4 *)(to + ((row0 + m) * N + at) * size) = w;
+                u32x4 *const place = (u32x4 *)(to + ((row0 + m) * N + at) * size);
+                if (m < M && at < N) {
+                    if constexpr (FORM == DWEIGHT) __builtin_nontemporal_store(w, place);
+                    else *place = w;
+                }
             }
         };
         if (!idle) {

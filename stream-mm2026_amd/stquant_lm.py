@@ -604,7 +604,7 @@ def route_forward(logits: torch.Tensor, k: int, *, renormalize: bool = False):
     ws = _workspace(_route_workspace(*head), z.device)
     _call(z.device, lm_lib().stq_route_forward,
           _ROUTE.pack(*head, int(renormalize), z.data_ptr(), z.stride(0), weights.data_ptr(), ids.data_ptr(), load.data_ptr(), 0, 0, 0, 0,
-                      ws.data_ptr(), ws.numel()))
+                      _ptr(ws), 0 if ws is None else ws.numel()))
     return weights, ids, load
 
 

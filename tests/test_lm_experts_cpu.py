@@ -44,8 +44,8 @@ def route(backward=False, **kw):
     (False, dict(w=0), "weights: null data pointer"),
     (False, dict(ids=P + 1), "ids must be aligned to 4 bytes"),
     (False, dict(load=P + 1), "load must be aligned to 4 bytes"),
-    (False, dict(ws=0), "workspace: null data pointer"),
-    (False, dict(wsn=100), "workspace needs 32768 bytes, got 100"),
+    (False, dict(n=100, ws=0), "workspace: null data pointer"),
+    (False, dict(n=100, wsn=100), "workspace needs 128 bytes, got 100"),
     (True, dict(dz=0), "dlogits: null data pointer"),
     (True, dict(dzs=7), "rows of dlogits must not overlap"),
     (True, dict(dw=P + 2), "dweights must be aligned to 4 bytes"),
@@ -70,7 +70,7 @@ def plan(**kw):
     (dict(rows=P + 2), "rows must be aligned to 4 bytes"),
     (dict(places=0), "places: null data pointer"),
     (dict(slots=100000), "workspace: null data pointer"),
-    (dict(slots=100000, ws=P, wsn=16), "workspace needs 500 bytes, got 16"),
+    (dict(slots=100000, ws=P, wsn=16), "workspace needs 980 bytes, got 16"),
 ])
 def test_plan_refusals(kw, msg):
     assert plan(**kw) == INVALID and msg in err()
