@@ -596,16 +596,31 @@ hipError_t launch_few(const ProductArgs &a, hipStream_t stream)
     return hipGetLastError();
 }
 
-// Tiles of 256 x 256 where an expert has many rows, of 128 x 128 (two workgroups a CU) where it has few, so that less of its
-// last tile is empty.  Measured (us, 256 against 128; forward, dx, dweight): 2048 rows an expert, 4096 x 11008: 1380, 1657,
-// 1378 against 1700, 1859, 1834; 768 x 2048: 68, 67, 54 against 67, 77, 66; 230 rows an expert, 1408 x 2048: 160, 170, 236
-// against 145, 148, 222.
+// Tiles of 256 x 256 where they are enough to fill most of the chip and, of rows, mostly full: 512 rows an expert, or 256 where
+// k is long enough to make up for a tile's beginning and end.  Tiles of 128 x 128 (two workgroups a CU) otherwise.
+// Measured, us, 256 against 128 (dx with its tokens' sums):
+//   8 experts of 4096 x 11008   forward              dx                   dweight
+//     128 rows an expert        217, 225             275, 215             197, 242
+//     256                       247, 295             318, 386             276, 343
+//     1024                      764, 888             928, 977             722, 952
+//   8 experts of 768 x 2048
+//     256                       21, 16               52, 31               15, 15
+//     1024                      42, 38               55, 41               31, 37
+//     2048                      67, 67               67, 77               53, 66
+//   60 experts of 1408 x 2048, skewed
+//     233                       156, 145             169, 147             172, 181
+//     273, evenly               170, 156             180, 154             150, not timed
+//     930                       394, 440             412, 424             583, 576
 template <int DT, int FORM, bool GATHER>
 hipError_t pick(const ProductArgs &a, hipStream_t stream)
 {
+    const int64_t in_tiles = (a.in + 255) / 256, out_tiles = (a.out + 255) / 256, rows_of_tiles = a.slots / 256 + a.experts / 2;
     if constexpr (FORM == FORWARD)
         if (a.slots <= 8 * (int64_t)a.experts) return launch_few<DT, GATHER>(a, stream);
-    if (a.slots >= 512 * (int64_t)a.experts) return launch<DT, FORM, GATHER, 256, 256, 2, 4, 64, 2>(a, stream);
+    const int64_t full = (FORM == FORWARD ? a.in : a.out) >= 4096 ? 256 : 512;
+    const bool large = FORM == DWEIGHT ? a.experts * in_tiles * out_tiles >= 128
+                                       : a.slots >= full * a.experts && rows_of_tiles * (FORM == FORWARD ? out_tiles : in_tiles) >= 192;
+    if (large) return launch<DT, FORM, GATHER, 256, 256, 2, 4, 64, 2>(a, stream);
     return launch<DT, FORM, GATHER, 128, 128, 2, 2, 64, 2>(a, stream);
 }
 

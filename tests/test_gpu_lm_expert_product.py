@@ -46,7 +46,7 @@ def test_against_64_bits(n, experts, k, din, dout, dtype, gather):
 
 
 # more tiles than workgroups, of both sizes, with tails of rows, columns and k; many rows an expert, one or none of them
-LARGE = [(4000, 4, 2, 1032, 4104), (3001, 2, 1, 72, 3080), (2500, 60, 4, 136, 4104), (9000, 1, 1, 520, 264), (700, 64, 1, 96, 2056), (513, 1, 1, 64, 64),
+LARGE = [(4000, 4, 2, 1032, 4104), (4000, 4, 2, 4104, 264), (3001, 2, 2, 4200, 4360), (13000, 3, 1, 2056, 1096), (3001, 2, 1, 72, 3080), (2500, 60, 4, 136, 4104), (9000, 1, 1, 520, 264), (700, 64, 1, 96, 2056), (513, 1, 1, 64, 64),
          (4100, 8, 1, 128, 192)]
 
 
