@@ -5,7 +5,8 @@
 // Squares and sums are doubles: no gradient that is a float overflows or vanishes in them, and the order of the sums does not
 // show in a float.  A tensor list travels as kernel arguments, 160 tensors a launch (no table to upload, so a call can
 // be captured).  Memory bound: the gradients are read twice, as their norm must be known before the first is written: GPT-2
-// small's in fp32 129 us for the norm (3.9 TB/s) and 170 for the scaling (5.9), 1.88 G elements of bf16 710 (5.3) and 1460 (5.2).
+// small's in fp32 95 us for the norm (5.2 TB/s) and 176 for the scaling (5.7), 1.88 G elements of bf16 680 (5.5) and 1444 (5.2).
+// Results are stored past the caches, which they do not fit: left there to be written back they slowed the next norm (129 us).
 #include "lm_clip.h"
 #include "lm_common.h"
 

@@ -11,7 +11,7 @@
 // A tile of 256 x 256 x 64 is 2048 cycles of products for the two waves of a SIMD.  Its operands' reads from LDS (192 KB) and the
 // loads' writes to it (64 KB) take nearly as long, so both run beside the products: loads go to LDS without registers in
 // between, operands are read a step ahead, and the next tile's loads are issued before this one's stores.  16384 rows of
-// 4096 x 11008 (bf16): forward 1380 us, 1.07 PFLOP/s; dx 1580, 0.93; dweight 1380, 1.07 (a library's dense products of the same
+// 4096 x 11008 (bf16): forward 1380 us, 1.07 PFLOP/s; dx 1570, 0.94; dweight 1370, 1.08 (a library's dense products of the same
 // sizes 1173, 1102, 1566); matrix units are busy for 61 to 66 % of the cycles, at the 1.7 GHz that the power allows.
 #pragma once
 #include "lm_common.h"
@@ -451,6 +451,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void product_kernel(ProductArgs a, 
                 const u32x4 w = *(const __attribute__((address_space(3))) u32x4 *)(mine + row * 128 + ((store_piece ^ (row >> 1 & 7)) << 4));
                 u32x4 *const place = (u32x4 *)(to + ((row0 + m) * N + at) * size);
                 if (m < M && at < N) {
+                    // (weight gradients wait for the optimizer: past the caches)
                     if constexpr (FORM == DWEIGHT) __builtin_nontemporal_store(w, place);
                     else *place = w;
                 }

@@ -7,8 +7,8 @@
 //
 // Rows are short (experts), so they live in registers: a row's experts are spread over 8 to 64 lanes, several rows a wave
 // where they are few.  What bounds these kernels is latency, launches above all: 8192 rows of 64 experts with 6 choices take 8.5
-// us for the choices (15 with exchanges through LDS and an exponential a choice), 4 for the load's sums, 13 for the plan
-// and 5.7 for the gradient, of 1 MB each way.
+// us for the choices (15 with exchanges through LDS and an exponential a choice), 4 for the load's sums, 10 for the plan
+// and 5.6 for the gradient, of 1 MB each way.
 #include "lm_common.h"
 #include "lm_expert.h"
 
