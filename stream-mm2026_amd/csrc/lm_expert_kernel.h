@@ -173,6 +173,7 @@ struct Operand {
     static constexpr int PIECES = ALONG ? BK / 8 : ROWS / 8;            // of 16 bytes in a row of the tile
     static constexpr int LOADS = BYTES / 16 / THREADS;
     static constexpr int STEP = THREADS / PIECES;                       // rows between a thread's loads
+    static_assert(STEP % (ALONG ? 16 : 4) == 0, "a thread's pieces are turned alike");
 
     static __device__ __forceinline__ int turn(int row) { return ALONG ? (BK == 64 ? row >> 1 & 7 : row >> 2 & 3) : (row & 3) << 2; }
     static __device__ __forceinline__ int row_of(int i) { return threadIdx.x / PIECES + i * STEP; }
@@ -257,67 +258,64 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void product_kernel(ProductArgs a, 
     };
 
     // Where each thread's pieces come from, k first, and the k that a piece stands for.  Rows of memory along k are clamped to
-    // the last, those across k to the first column.
-    const char *pa[OpA::LOADS], *pb[OpB::LOADS];
+    // the last, those across k to the first column (and lie STEP rows apart: one pointer for all of a thread's pieces).
+    const char *pa[FORM == DWEIGHT ? 1 : OpA::LOADS], *pb[FORM == FORWARD ? OpB::LOADS : 1];
     int sa[OpA::LOADS], sb[OpB::LOADS];
 #pragma unroll
     for (int i = 0; i < OpA::LOADS; i++) sa[i] = FORM == DWEIGHT ? OpA::row_of(i) : OpA::piece_of(i) * 8;
 #pragma unroll
     for (int i = 0; i < OpB::LOADS; i++) sb[i] = FORM == FORWARD ? OpB::piece_of(i) * 8 : OpB::row_of(i);
-    // Rows of the sorted buffer, or with GATHER the slots there, on their way: FORWARD the rows of a tile of A, DWEIGHT
-    // those of the k that are fetched next.  (A slot becomes a token only where it is needed: here it would have to arrive
-    // first, behind all loads that were issued before it.)
+    // With GATHER, the slots of the rows that are needed next, on their way: FORWARD those of a tile of A, DWEIGHT those of the k
+    // that is fetched next.  (A slot becomes a token only where it is needed: here it would have to arrive first, behind
+    // all loads that were issued before it.)
+    constexpr bool AHEAD = GATHER && FORM != DX;
     int ahead[FORM == DWEIGHT ? OpB::LOADS : OpA::LOADS];
+    auto row_of_a = [&](const Tile &t, int i) { return t.first + min(t.m * BM + OpA::row_of(i), t.last - t.first - 1); };
     auto look_ahead = [&](const Tile &t, int K, int k0) {
-        if constexpr (FORM == DWEIGHT) {
+        if constexpr (AHEAD && FORM == DWEIGHT) {
             if (K == 0) return;
 #pragma unroll
-            for (int i = 0; i < OpB::LOADS; i++) {
-                const int r = t.first + min(k0 + sb[i], K - 1);
-                ahead[i] = GATHER ? a.rows[r] : r;
-            }
-        } else {
+            for (int i = 0; i < OpB::LOADS; i++) ahead[i] = a.rows[t.first + min(k0 + sb[i], K - 1)];
+        } else if constexpr (AHEAD) {
 #pragma unroll
-            for (int i = 0; i < OpA::LOADS; i++) {
-                const int r = t.first + min(t.m * BM + OpA::row_of(i), t.last - t.first - 1);
-                ahead[i] = GATHER && FORM == FORWARD ? a.rows[r] : r;
-            }
+            for (int i = 0; i < OpA::LOADS; i++) ahead[i] = a.rows[row_of_a(t, i)];
         }
     };
-    auto source = [&](int i) { return GATHER ? (int64_t)token_of(a, ahead[i]) : (int64_t)ahead[i]; };
     auto aim = [&](const Tile &t) {
         const int m0 = t.m * BM, n0 = t.n * BN;
         const char *const weight = (const char *)a.weight + (t.expert == a.experts ? 0 : (int64_t)t.expert * a.weight_expert_stride) * 2;
+        if constexpr (FORM == DWEIGHT) {
+            const int col = m0 + OpA::piece_of(0) * 8;
+            pa[0] = (const char *)a.dy + ((t.first + sa[0]) * a.dy_stride + (col < a.out ? col : 0)) * 2;
+        } else
 #pragma unroll
-        for (int i = 0; i < OpA::LOADS; i++) {
-            if constexpr (FORM == DWEIGHT) {
-                const int col = m0 + OpA::piece_of(i) * 8;
-                pa[i] = (const char *)a.dy + ((t.first + sa[i]) * a.dy_stride + (col < a.out ? col : 0)) * 2;
-            } else if constexpr (FORM == FORWARD) pa[i] = (const char *)a.x + (source(i) * a.x_stride + sa[i]) * 2;
-            else pa[i] = (const char *)a.dy + (ahead[i] * a.dy_stride + sa[i]) * 2;
-        }
+            for (int i = 0; i < OpA::LOADS; i++)
+                if constexpr (AHEAD) pa[i] = (const char *)a.x + (token_of(a, ahead[i]) * a.x_stride + sa[i]) * 2;
+                else if constexpr (FORM == FORWARD) pa[i] = (const char *)a.x + (row_of_a(t, i) * a.x_stride + sa[i]) * 2;
+                else pa[i] = (const char *)a.dy + (row_of_a(t, i) * a.dy_stride + sa[i]) * 2;
+        if constexpr (FORM == FORWARD) {
 #pragma unroll
-        for (int i = 0; i < OpB::LOADS; i++) {
-            if constexpr (FORM == FORWARD) pb[i] = weight + (min(n0 + OpB::row_of(i), N - 1) * a.weight_row_stride + sb[i]) * 2;
-            else {
-                const int col = n0 + OpB::piece_of(i) * 8, at = col < N ? col : 0;
-                if constexpr (FORM == DX) pb[i] = weight + (sb[i] * a.weight_row_stride + at) * 2;
-                else pb[i] = (const char *)a.x + at * 2;
-            }
+            for (int i = 0; i < OpB::LOADS; i++) pb[i] = weight + (min(n0 + OpB::row_of(i), N - 1) * a.weight_row_stride + sb[i]) * 2;
+        } else {
+            const int col = n0 + OpB::piece_of(0) * 8, at = col < N ? col : 0;
+            if constexpr (FORM == DX) pb[0] = weight + (sb[0] * a.weight_row_stride + at) * 2;
+            else pb[0] = (const char *)a.x + ((AHEAD ? 0 : (t.first + sb[0]) * a.x_stride) + at) * 2;
         }
     };
     // (what lies behind the end of k is ZEROS, so that no step of the loop branches)
     auto fetch = [&](int K, int k0, int buffer) {
         lds_char *la = (lds_char *)lds + buffer * (OpA::BYTES + OpB::BYTES), *lb = la + OpA::BYTES;
-        const int64_t ka = FORM == DWEIGHT ? k0 * a.dy_stride * 2 : (int64_t)k0 * 2;
-        const int64_t kb = FORM == FORWARD ? (int64_t)k0 * 2 : k0 * a.weight_row_stride * 2;
 #pragma unroll
-        for (int i = 0; i < OpA::LOADS; i++) OpA::load(la, wave, i, k0 + sa[i] < K ? pa[i] + ka : zeros);
+        for (int i = 0; i < OpA::LOADS; i++) {
+            const char *p = pa[FORM == DWEIGHT ? 0 : i];
+            p += FORM == DWEIGHT ? (k0 + i * OpA::STEP) * a.dy_stride * 2 : (int64_t)k0 * 2;
+            OpA::load(la, wave, i, k0 + sa[i] < K ? p : zeros);
+        }
 #pragma unroll
         for (int i = 0; i < OpB::LOADS; i++) {
-            const char *p = pb[i];
-            if constexpr (FORM == DWEIGHT) p += source(i) * a.x_stride * 2;
-            else p += kb;
+            const char *p = pb[FORM == FORWARD ? i : 0];
+            if constexpr (FORM == DWEIGHT) p += (AHEAD ? token_of(a, ahead[i]) : k0 + i * OpB::STEP) * a.x_stride * 2;
+            else p += FORM == FORWARD ? (int64_t)k0 * 2 : (k0 + i * OpB::STEP) * a.weight_row_stride * 2;
             OpB::load(lb, wave, i, k0 + sb[i] < K ? p : zeros);
         }
     };
@@ -494,6 +492,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void product_kernel(ProductArgs a, 
         }
         // (stores that no lane makes are not issued: of a tile that is not full they are waited for)
         behind = m0 + BM <= M && n0 + BN <= N ? wide ? MI * NI * 4 : MI * 4 : 0;
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
