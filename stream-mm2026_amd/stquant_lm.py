@@ -663,8 +663,8 @@ def expert_plan(ids: torch.Tensor, experts: int) -> ExpertPlan:
     """The slots of ``ids`` [..., k] sorted by expert, those of one expert in their order.  Ids outside
     [0, experts) (-1) belong to none."""
     ic = _index_code("ids", ids)
-    if ids.dim() < 1:
-        _fail("ids must be [..., k]")
+    if ids.dim() < 1 or ids.shape[-1] == 0:
+        _fail(f"ids must be [..., k] with k > 0, got {tuple(ids.shape)}")
     _same_device(ids)
     ids = ids.contiguous()
     n = ids.numel()
@@ -682,7 +682,7 @@ def _check_plan(plan: ExpertPlan, near: torch.Tensor) -> None:
     for name, t in (("rows", rows), ("places", places), ("offsets", offsets)):
         if t.dtype != torch.int32 or not t.is_contiguous():
             _fail(f"the plan's {name} must be dense int32, got {t.dtype}")
-    if places.dim() < 1 or rows.shape != (places.numel(),) or offsets.dim() != 1 or offsets.numel() < 2:
+    if places.dim() < 1 or places.shape[-1] == 0 or rows.shape != (places.numel(),) or offsets.dim() != 1 or offsets.numel() < 2:
         _fail(f"not a plan: rows {tuple(rows.shape)}, places {tuple(places.shape)}, offsets {tuple(offsets.shape)}")
     _same_device(near, rows=rows, places=places, offsets=offsets)
 

@@ -218,6 +218,9 @@ def test_python_refusals():
         (lambda: lm.expert_product_forward(f, w, p), "x and weight must both be bfloat16 or both float16"),
         (lambda: lm.expert_product_forward(h, w, p._replace(rows=p.rows.long())), "the plan's rows must be dense int32"),
         (lambda: lm.expert_product_forward(h, w, p._replace(rows=p.rows[:7])), "not a plan"),
+        # no choice a token: its gradient would never be written
+        (lambda: lm.expert_product_forward(h, w, lm.ExpertPlan(p.rows[:0], i[:, :0].contiguous(), p.offsets), gather=True), "not a plan"),
+        (lambda: lm.expert_plan(i[:, :0], 3), r"ids must be \[..., k\] with k > 0"),
         (lambda: lm.expert_product_forward(h, w, p), "tensors must be CUDA"),
         (lambda: lm.expert_combine_forward(f.double(), None, p), "y must be float32, bfloat16 or float16"),
         (lambda: lm.expert_combine_forward(f, None, p), "tensors must be CUDA"),
