@@ -216,7 +216,8 @@ int stq_expert_plan_sort(const stq_expert_plan *a, void *stream);
  * an expert without rows gets dW = 0.  Sums are fp32, results rounded once.
  * BFloat16 or Half; in and out multiples of 8 up to 2^20; x, weight, dy: rows strided, 16-byte aligned, strides multiples
  * of 8; y, dx, dweight dense and aligned likewise.  dweight_dtype: dtype or Float.  backward: dx or dweight may be null (not wanted).
- * slots up to 2^30, and slots / 128 + experts times the tiles of 128 of the wider of in and out up to 2^23.
+ * slots up to 2^30.  In tiles of 128 x 128, the rows that a pass writes (slots / 128, rounded down, times the tiles of out,
+ * or of in for dx) and the weights have up to 2^23 each.
  * workspace: backward with dx and k > 0, stq_expert_product_workspace(a) bytes.
  */
 typedef struct stq_expert_product {

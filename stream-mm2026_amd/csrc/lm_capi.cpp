@@ -387,6 +387,10 @@ int check_pieces(const char *name, const void *p, int64_t stride)
     return STQ_OK;
 }
 
+// Kernels count tiles in 32 bits.  2^23 of 128 x 128 are results of 256 GiB in 16 bits; those that are not full (one an expert,
+// and one of the rows of none, for each of up to 2^13 columns of tiles) come on top and stay below 2^23 too.
+constexpr int64_t PRODUCT_TILES = 1 << 23;
+
 int check_product_sizes(const stq_expert_product *a)
 {
     if (!a) return bad("null arguments");
@@ -400,15 +404,20 @@ int check_product_sizes(const stq_expert_product *a)
     if (a->k) CHECK(check_size("tokens", a->tokens, 0, lm::SLOT_MAX));
     if (a->k && a->tokens * a->k != a->slots)
         return fail(STQ_ERR_INVALID, "slots (%lld) must be tokens (%lld) times k (%lld)", (long long)a->slots, (long long)a->tokens, (long long)a->k);
-    // (a launch has fewer than 2^32 threads along a dimension)
-    const int64_t wide = ((a->in > a->out ? a->in : a->out) + 127) / 128, narrow = ((a->in > a->out ? a->out : a->in) + 127) / 128;
-    CHECK(check_size("tiles of rows", (a->slots / 128 + a->experts + 1) * wide, 0, 1 << 23));
-    return check_size("tiles of weights", a->experts * wide * narrow, 0, 1 << 23);
+    return check_size("tiles of weights", a->experts * ((a->in + 127) / 128) * ((a->out + 127) / 128), 0, PRODUCT_TILES);
+}
+
+// The full tiles of the rows that a pass writes: y of `out` columns, dx of `in` (dweight writes none).
+int check_product_rows(const stq_expert_product *a, bool backward)
+{
+    if (backward && !a->dx) return STQ_OK;
+    return check_size("tiles of rows", a->slots / 128 * (((backward ? a->in : a->out) + 127) / 128), 0, PRODUCT_TILES);
 }
 
 int check_product(const stq_expert_product *a, bool backward)
 {
     CHECK(check_product_sizes(a));
+    CHECK(check_product_rows(a, backward));
     CHECK(check_ptr("offsets", a->offsets, 4));
     CHECK(check_ptr("weight", a->weight, 16));
     if (a->weight_expert_stride % 8 || a->weight_row_stride % 8 || a->weight_expert_stride < 0 || a->weight_row_stride < 0)
@@ -732,7 +741,7 @@ int stq_expert_plan_sort(const stq_expert_plan *a, void *stream)
 
 int64_t stq_expert_product_workspace(const stq_expert_product *a)
 {
-    if (check_product_sizes(a) != STQ_OK) return -1;
+    if (check_product_sizes(a) != STQ_OK || check_product_rows(a, true) != STQ_OK) return -1;
     return lm::product_workspace(product_args(a));
 }
 

@@ -113,3 +113,31 @@ def test_clipping():
     for got, value, u in ((g[0], 2.0 ** -10, BF16), (g[-6], 2.0 ** -10, BF16), (g[-1], 3.0, BF16), (small[-1], 1.0, torch.float32)):
         assert abs(float(got) - value * c) <= value * c * (ref.U[u] + 2.0 ** -22)
     assert bool((g[:-5] == g[0]).all())
+
+
+def test_wide_rows_of_narrow_results():
+    """131072 slots of 2^20 columns: what is counted against the limits is what a pass writes.  Whole numbers, whose sums fp32 holds
+    exactly, so that each result is the exact sum rounded once."""
+    tokens, k, experts, din, dout = 2048, 64, 3, 1 << 20, 8
+    g = ref.gen(11)
+    few = lambda *shape: torch.randint(-1, 2, shape, device="cuda", generator=g, dtype=torch.int8).to(BF16)  # noqa: E731
+    x, w, dy = few(tokens, din), few(experts, dout, din), few(tokens * k, dout)
+    ids = torch.randint(0, experts, (tokens, k), device="cuda", generator=g, dtype=torch.int32)
+    plan = lm.expert_plan(ids, experts)
+    y = lm.expert_product_forward(x, w, plan, gather=True)
+    dx, dw = lm.expert_product_backward(dy, x, w, plan, gather=True, inputs=False)
+    assert dx is None
+    owner, token = ids.view(-1)[plan.rows.long()].long(), plan.rows.long() // k
+    # each token's gradient of each expert, and each token through each expert
+    sums = torch.zeros(experts, tokens, dout, dtype=torch.float64, device="cuda")
+    sums.index_put_((owner, token), dy.double(), accumulate=True)
+    through = torch.zeros(experts, tokens, dout, dtype=torch.float64, device="cuda")
+    for at in range(0, din, 1 << 16):
+        part = x[:, at:at + (1 << 16)].double()
+        for e in range(experts):
+            through[e] += part @ w[e, :, at:at + (1 << 16)].double().t().contiguous()
+            want = sums[e].t().contiguous() @ part
+            assert float(want.abs().max()) < 1 << 24
+            assert torch.equal(dw[e, :, at:at + (1 << 16)], want.to(BF16)), (e, at)
+    assert float(through.abs().max()) < 1 << 24
+    assert torch.equal(y, through[owner, token].to(BF16))

@@ -203,6 +203,23 @@ def test_limits_of_a_launch():
     assert product(slots=1 << 23, k=0, dout=11008, din=4096, x=0) == INVALID and "x: null data pointer" in err()
 
 
+def test_limits_go_by_what_a_pass_writes():
+    """Tiles are counted of the rows that a pass writes: y is as wide as out, dx as in, and a call without dx has none.  Wide inputs of
+    narrow results, and runs of 2^30 rows, are inside (refused further on, for a null pointer, so that nothing runs)."""
+    L = _capi.lm_lib()
+    wide = dict(slots=1 << 24, tokens=1 << 21, k=8, din=8192, dout=64, x=0)
+    for backward, kw in ((False, wide), (False, wide | dict(slots=131072, tokens=2048, k=64, din=1 << 20, dout=8)), (False, wide | dict(slots=1 << 30, k=0, din=8)),
+                         (True, wide | dict(dx=0)), (True, wide | dict(slots=1 << 30, k=0, din=64, dout=8192))):
+        assert product(backward, **kw) == INVALID and "x: null data pointer" in err()
+    for backward, kw in ((False, wide | dict(din=64, dout=8200)), (True, wide | dict(din=8200)), (True, wide | dict(din=8200, k=0))):
+        assert product(backward, **kw) == INVALID and "tiles of rows must be 0 to 8388608, got 8519680" in err()
+    need = lambda **kw: L.stq_expert_product_workspace(lm._PRODUCT.pack(*(PRODUCT | wide | kw).values()))  # noqa: E731
+    assert need(dx=0, din=8200) == 0 and need(din=64, dout=8200) == (1 << 24) * 64 * 4
+    assert need(din=8200) == -1 and "tiles of rows" in err()
+    # counted in 32 bits: full tiles, one that is not full for each expert and the rows of none, and a step beyond the last
+    assert (1 << 23) + (512 + 1) * (1 << 13) + 512 < 1 << 32
+
+
 def test_python_refusals():
     f, i = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int32)
     h = f.bfloat16()
