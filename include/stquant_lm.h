@@ -21,7 +21,9 @@
 extern "C" {
 #endif
 
-#define STQ_LM_ABI_VERSION 2
+/* Of the structs below and what their calls mean; added structs and entries leave it as it is.  (2 was the same as 1
+ * with more entries: the next is 3.) */
+#define STQ_LM_ABI_VERSION 1
 
 /*
  * out[i, :] = scale * weight[tokens[i], :]; a token outside [0, vocab) gives a row of NaN.

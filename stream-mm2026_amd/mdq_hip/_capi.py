@@ -83,7 +83,7 @@ LM_SYMBOLS = (
     "stq_clip_grads",
     "stq_lm_abi_version",
 )
-LM_ABI_VERSION = 2
+LM_ABI_VERSION = 1
 
 # STQ_ABI_VERSION of include/stquant_hip.h this package is written against
 ABI_VERSION = 4

@@ -48,6 +48,14 @@ def test_packed_structs_follow_the_header(name, packed):
     assert flat == fields(name) and packed.size == 8 * len(flat)
 
 
+def test_added_entries_keep_the_version():
+    """A caller that was built when the header had these structs alone compares versions for equality: the library serves it."""
+    assert {n: fields(n) for n in ("stq_embedding", "stq_embedding_grad", "stq_norm_residual", "stq_attention", "stq_distill")} == {
+        "stq_embedding": "q" * 10 + "d", "stq_embedding_grad": "q" * 15 + "d", "stq_norm_residual": "q" * 15 + "dd" + "q" * 16,
+        "stq_attention": "q" * 9 + "d" + "q" * 37, "stq_distill": "q" * 12 + "dd" + "q" * 5}
+    assert _capi.lm_lib().stq_lm_abi_version() == 1
+
+
 def embed(**kw):
     a = dict(tokens=P, tdt=9, n=4, vocab=10, dim=8, weight=P, wdt=0, ws=8, out=P, odt=0, scale=1.0) | kw
     return _capi.lm_lib().stq_embedding_forward(lm._EMBED.pack(*a.values()), None)
