@@ -850,6 +850,9 @@ def _grad_list(grads, out):
     into = grads if out is None else list(out)
     if len(into) != len(grads):
         _fail(f"out must be {len(grads)} tensors, got {len(into)}")
+    for t in grads if out is None else (*grads, *into):
+        if t is None:
+            _fail("gradients must be tensors, got None: parameters without a gradient are left out")
     flat = []
     index = grads[0].get_device() if grads else -1
     if grads and index < 0:
@@ -893,8 +896,8 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, norm: Optional
     """Scales the gradients in place by ``min(1, max_norm / (norm + 1e-6))`` and returns their :func:`grad_norm`, without
     a synchronisation.
 
-    ``grads``: dense fp32, bf16 or fp16 tensors of one device, apart from each other in memory.  ``out``: tensors like
-    them that take the result in their place.  ``norm``: a fp32 scalar to scale by, e.g. one formed over several ranks.
+    ``grads``: dense fp32, bf16 or fp16 tensors of one device, apart from each other in memory (a parameter without a gradient
+    is left out).  ``out``: tensors like them that take the result in their place.  ``norm``: a fp32 scalar to scale by, e.g. one formed over several ranks.
     A norm of NaN makes every gradient NaN, an infinite one 0 (its infinite ones NaN)."""
     grads, into, packed = _grad_list(grads, out)
     if not grads:

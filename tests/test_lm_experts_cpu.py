@@ -1,14 +1,16 @@
 """Routing, expert products and clipping without a GPU: the packed structs have the header's layout, and bad arguments are
 reported before any device work (the pointers below are never dereferenced)."""
 import ctypes
+import os
 import struct
+import types
 
 import pytest
 import torch
 
 import stquant_lm as lm
 from mdq_hip import _capi
-from test_lm_cpu import INVALID, P, err, fields
+from test_lm_cpu import INVALID, P, ROOT, err, fields
 
 
 @pytest.mark.parametrize("name,packed", [("stq_route", lm._ROUTE), ("stq_expert_plan", lm._PLAN), ("stq_expert_product", lm._PRODUCT),
@@ -247,6 +249,21 @@ def test_python_refusals():
     ]:
         with pytest.raises(RuntimeError, match=msg):
             call()
+
+
+def test_gradients_that_are_none():
+    """A parameter that took no part in the step has none: said so, not an AttributeError, and the README's example leaves it out."""
+    f = torch.zeros(4, 8)
+    for call in (lambda: lm.grad_norm([None]), lambda: lm.grad_norm([f, None]), lambda: lm.clip_grads([None, f], 1.0), lambda: lm.clip_grads([f], 1.0, out=[None])):
+        with pytest.raises(RuntimeError, match="must be tensors, got None"):
+            call()
+    readme = open(os.path.join(ROOT, "README.md")).read()
+    lines = [line.split("#")[0].split("=", 1)[1] for line in readme.splitlines() if "lm.clip_grads(" in line]
+    model, seen = torch.nn.ParameterList([torch.zeros(3), torch.zeros(5)]), []
+    model[1].grad = torch.ones(5)
+    for line in lines:
+        eval(line, {"model": model, "lm": types.SimpleNamespace(clip_grads=lambda grads, most: seen.append(list(grads)))})
+    assert lines and all(len(s) == 1 and s[0] is model[1].grad for s in seen)
 
 
 def test_dense():
