@@ -132,6 +132,7 @@ def step_loss(model: Decoder, tokens: torch.Tensor, targets, *, temperature: flo
         logits.backward(dz)
     else:
         torch.autograd.backward([logits, balance * model.uneven], [dz, None])
+        model.uneven = model.uneven.detach()         # (the number: its graph would live until the next call)
     return loss.mean()
 
 

@@ -1,5 +1,6 @@
 """Routing, expert products, their combination and clipping together, as ``distill_pretrain.py`` uses them: one step of a
 sparse decoder against the same model in plain fp32 torch, training with the 4-bit optimizer, graphs and streams."""
+import copy
 import math
 
 import pytest
@@ -74,6 +75,16 @@ def test_one_step_against_plain_torch(monkeypatch):
     for n, p in model.named_parameters():
         off = float((got[n] - p.grad).norm() / p.grad.norm())
         assert off <= 0.055, (n, off)
+
+
+def test_a_step_leaves_no_graph_behind():
+    """A model that still held the step's graph could not be copied, and a backward pass of its weights not be captured."""
+    model, teacher = dp.Decoder(seed=1, **SMALL), dp.Decoder(seed=2, **SMALL)
+    tokens = torch.randint(0, 515, (2, 30), device="cuda", generator=ref.gen(0))
+    dp.step_loss(model, tokens, dp.teach(teacher, tokens, 16), temperature=2.0, alpha=0.6)
+    assert model.uneven.grad_fn is None and not model.uneven.requires_grad and float(model.uneven) > 0.0
+    twin = copy.deepcopy(model)
+    assert all(torch.equal(a, b) for a, b in zip(twin.parameters(), model.parameters()))
 
 
 def test_training_with_the_low_bit_optimizer_and_clipping():
