@@ -44,6 +44,18 @@ def test_against_64_bits(sizes, dtype, apart):
     check(grads, 0.3 * norm, out=[torch.full_like(g, 7.0) for g in grads] if apart else None)
 
 
+@pytest.mark.parametrize("count", [159, 160, 161, 319, 320, 321])
+@pytest.mark.parametrize("empty", [None, 0, 159, 160])
+@pytest.mark.parametrize("apart", [False, True])
+def test_lists_that_end_at_a_launch(count, empty, apart):
+    """A launch holds 160 tensors (empty ones take no place): lists around one and two of them, with an empty tensor at the cut."""
+    sizes = [1 + 37 * i % 101 for i in range(count)]
+    if empty is not None and empty < count:
+        sizes[empty] = 0
+    grads = [t for i, n in enumerate(sizes) for t in tensors([n], (F32, BF16, F16)[i % 3], seed=i)]
+    check(grads, 0.05, out=[torch.full_like(g, 7.0) for g in grads] if apart else None)
+
+
 def test_mixed_types():
     grads = [t for d in (F32, BF16, F16) for t in tensors([1000, 33, 70000], d, seed=3)]
     check(grads, 0.1)

@@ -137,6 +137,15 @@ def test_fp32_weight_gradients(n, experts, k, din, dout):
     check(ids, x, w, dy, True, dtype=torch.float32)
 
 
+@pytest.mark.parametrize("n,experts,k,din,dout", [(4000, 4, 2, 1032, 4104), (3001, 2, 2, 4200, 4360), (700, 64, 1, 264, 520), (6000, 130, 1, 256, 256)])
+@pytest.mark.parametrize("dtype,gather,skew", [(BF16, True, True), (F16, False, False)])
+def test_fp32_weight_gradients_in_large_tiles(n, experts, k, din, dout, dtype, gather, skew):
+    """More tiles than workgroups, full ones and cut ones, experts of no row among them."""
+    ids, x, w, dy = operands(n, experts, k, din, dout, dtype, gather, skew=skew, absent=0.1 if skew else 0.0)
+    ids[ids == experts - 1] = 0
+    check(ids, x, w, dy, gather, dtype=torch.float32)
+
+
 def test_parts_of_the_backward_pass():
     ids, x, w, dy = operands(200, 6, 2, 72, 104, F16, True)
     plan = lm.expert_plan(ids, 6)

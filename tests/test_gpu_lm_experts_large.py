@@ -59,6 +59,36 @@ def test_gathered_products():
     ref.within("y", out[-500:], want[0][at], (din + 1) * er.EPS32 * want[1][at])
 
 
+def test_gathered_products_backward():
+    """The sorted rows' gradients (fp32) and the tokens are more than 2^31 elements each."""
+    tokens, k, din, dout = 300_001, 2, 7200, 64
+    x, w = big(tokens, din, BF16, 12), ref.randn(ref.gen(13), 3, dout, din, std=din ** -0.5, dtype=BF16)
+    ids = torch.stack([torch.arange(tokens, device="cuda") % 2, torch.arange(tokens, device="cuda") // 150_000 + 1], 1).int()       # (0 or 1, then 1, 2 or none)
+    plan = lm.expert_plan(ids, 3)
+    dy = ref.randn(ref.gen(14), tokens * k, dout, dtype=BF16)
+    dx, dw = lm.expert_product_backward(dy, x, w, plan, gather=True)
+    g = dy[plan.places.long()]                                # [tokens, k, dout]
+    there = (ids < 3).double()
+    for rows in (slice(0, 300), slice(tokens - 600, tokens)):
+        s, m = (torch.zeros(x[rows].shape, dtype=torch.float64, device="cuda") for _ in range(2))
+        for j in range(k):
+            for e in range(3):
+                p = g[rows, j].double() * (ids[rows, j] == e).double()[:, None]
+                s += p @ w[e].double()
+                m += p.abs() @ w[e].double().abs()
+        ref.within("dx", dx[rows], s, (dout + k + 1) * er.EPS32 * m)
+    for e in range(3):
+        s, m = (torch.zeros(dout, din, dtype=torch.float64, device="cuda") for _ in range(2))
+        for at in range(0, tokens, 20_000):
+            part = x[at:at + 20_000].double()
+            for j in range(k):
+                p = (g[at:at + 20_000, j].double() * (ids[at:at + 20_000, j] == e).double()[:, None]).t().contiguous()
+                s += p @ part
+                m += p.abs() @ part.abs()
+        ref.within(f"dweight {e}", dw[e], s, (int((ids == e).sum()) + 1) * er.EPS32 * m)
+    assert 0 < int(there.sum()) < tokens * k
+
+
 def test_combination():
     n, k, dim = 150_001, 2, 7200
     assert n * k * dim > 1 << 31

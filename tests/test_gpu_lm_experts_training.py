@@ -105,6 +105,26 @@ def test_training_with_the_low_bit_optimizer_and_clipping():
         assert before > 0.05 and abs(after - 0.05 * before / (before + 1e-6)) <= 1e-5 * 0.05
 
 
+def test_every_expert_learns(monkeypatch):
+    """Each expert's matrices and each router have a gradient in every step, and all of them differ from where they began."""
+    models, made, clip = [], dp.Decoder, lm.clip_grads
+
+    def spy(grads, most):
+        grads = list(grads)
+        for g in grads:
+            if g.dim() == 3:
+                assert bool((g.flatten(1).abs().amax(1) > 0).all())
+        assert sum(g.dim() == 3 for g in grads) == 4
+        return clip(grads, most)
+    monkeypatch.setattr(dp, "Decoder", lambda **k: (models.append(made(**k)) or models[-1]))
+    monkeypatch.setattr(lm, "clip_grads", spy)
+    dp.train(steps=3, warmup=1, batch=4, seq_len=64, lr=2e-3, k=16, vocab_used=64, max_grad_norm=0.05, **SMALL)
+    model, before = models[0], made(seed=42, **SMALL)
+    for name in ("up", "down", "router"):
+        for a, b in zip(getattr(model, name), getattr(before, name)):
+            assert bool(((a - b).flatten(1).abs().amax(1) > 0).all()), name
+
+
 def layer(x, logits, up, down, k=2):
     w, ids, load = lm.route(logits, k, renormalize=True)
     plan = lm.expert_plan(ids, up.shape[0])
@@ -196,3 +216,23 @@ def test_two_streams_at_once():
     for i in range(2):
         for g in got[i]:
             assert torch.equal(g[0], want[i][0]) and torch.equal(g[1], want[i][1]) and float(g[2]) == float(got[i][0][2])
+
+
+def test_norms_on_two_streams_at_once():
+    """Against norms formed beforehand, one at a time."""
+    lists = [[ref.randn(ref.gen(i), n + 7 * i, dtype=d) for n in (5, 40_000, 300_001) for d in (torch.float32, torch.bfloat16)] for i in range(2)]
+    want = [er.clip(g, 1.0)[0] for g in lists]
+    streams = [torch.cuda.Stream() for _ in lists]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                out = [torch.empty_like(g) for g in lists[i]]
+                got[i].append((lm.clip_grads(lists[i], 1.0, out=out), lm.grad_norm(lists[i]), out))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for norm, again, out in got[i]:
+            assert abs(float(norm) - want[i]) <= want[i] * (2.0 ** -24 + 2.0 ** -40) and float(again) == float(norm)
+            for o, g in zip(out, er.clip(lists[i], 1.0)[1]):
+                ref.within("gradient", o, g, 2.0 ** -23 * g.abs())
