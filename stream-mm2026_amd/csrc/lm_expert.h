@@ -73,7 +73,7 @@ struct ProductArgs {
     const void *dy;                      // [slots, out]
     int64_t dy_stride;
     void *dx;                            // [slots, in] (k > 0: [tokens, in]) dense, or null
-    float *scratch;                      // k > 1: [slots, in]
+    float *scratch;                      // k > 0, where dx is wanted: [slots, in]
     void *dweight;                       // [experts, out, in] dense, or null
     int dweight_f32;
 };

@@ -164,18 +164,22 @@ __device__ __forceinline__ int64_t source_row(const ProductArgs &a, int r)
     else return r;
 }
 
-// One operand's LDS tile of ROWS x BK.  (No bank conflicts in any of the three forms but for the results' way out.)  ALONG: its memory is dense along k (a row of the tile is a row of memory, BK of its
+// One operand's LDS tile of ROWS x BK.  ALONG: its memory is dense along k (a row of the tile is a row of memory, BK of its
 // elements); otherwise dense across (a row of the tile is one k, ROWS elements).  16-byte pieces are XOR-ed with their row, so
 // that the lanes of a read fall on different banks; loads write LDS in lane order, so the lanes' addresses are permuted instead.
+// The conflicts that are counted go with the results' way out, which costs about twice its accesses: they are 2 % of the LDS
+// cycles with 64 steps of k a tile (forward of 4096 x 11008), 9 % with 12 (forward of 768 x 2048), 18 % with four (dweight
+// of 60 skewed experts).
 template <int ROWS, bool ALONG, int THREADS, int BK>
 struct Operand {
+    static_assert(BK == 64, "turn");
     static constexpr int BYTES = ROWS * BK * 2;
     static constexpr int PIECES = ALONG ? BK / 8 : ROWS / 8;            // of 16 bytes in a row of the tile
     static constexpr int LOADS = BYTES / 16 / THREADS;
     static constexpr int STEP = THREADS / PIECES;                       // rows between a thread's loads
     static_assert(STEP % (ALONG ? 16 : 4) == 0, "a thread's pieces are turned alike");
 
-    static __device__ __forceinline__ int turn(int row) { return ALONG ? (BK == 64 ? row >> 1 & 7 : row >> 2 & 3) : (row & 3) << 2; }
+    static __device__ __forceinline__ int turn(int row) { return ALONG ? row >> 1 & 7 : (row & 3) << 2; }
     static __device__ __forceinline__ int row_of(int i) { return threadIdx.x / PIECES + i * STEP; }
     static __device__ __forceinline__ int piece_of(int i) { return (threadIdx.x % PIECES) ^ turn(row_of(i)); }
 
@@ -449,7 +453,9 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void product_kernel(ProductArgs a, 
                 const u32x4 w = *(const __attribute__((address_space(3))) u32x4 *)(mine + row * 128 + ((store_piece ^ (row >> 1 & 7)) << 4));
                 u32x4 *const place = (u32x4 *)(to + ((row0 + m) * N + at) * size);
                 if (m < M && at < N) {
-                    // (weight gradients wait for the optimizer: past the caches)
+                    // (past the caches: left there they push out the operands.  60 skewed experts, 692 MB in fp32: 380 us against
+                    // 485, with a clip_grads of them behind it 816 against 875; 25 MB in bf16, which a cache could keep for that
+                    // clip_grads: 78 against 77)
                     if constexpr (FORM == DWEIGHT) __builtin_nontemporal_store(w, place);
                     else *place = w;
                 }
@@ -516,7 +522,9 @@ hipError_t launch(const ProductArgs &a, hipStream_t stream)
 // Forward for few rows an expert (decoding): the weights are read once and bound it.  A workgroup has 16 rows and 32 columns;
 // its four waves share k, 64 at a time, read their operands of 16x16x32 products straight from memory (a line of each weight
 // row at a time, FLY of them in flight) and add their sums in LDS in the order of the waves.  1 token, 2 of 8 experts of
-// 4096 x 11008: 29.8 us a call, 6.0 TB/s (tiles of 128: 65).  Up to 8 rows an expert on average: at 8 153 us against 163 with
+// 4096 x 11008: 38 to 40 us, 4.5 TB/s, with other weights read in between; 29.8 where the last-level cache still holds them in part
+// (tiles of 128: 65).  Narrow experts are bound by the dependent reads ahead of the weights (row counts, slot, row), which one
+// trip of loads follows: 37 tokens, 2 of 16 experts of 768 x 2048, 12.5 us for about 40 MB.  Up to 8 rows an expert on average: at 8 153 us against 163 with
 // tiles of 128 for 4096 x 11008, at 16 205 against 163.
 constexpr int FEW_M = 16, FEW_N = 32;
 
@@ -611,6 +619,7 @@ hipError_t launch_few(const ProductArgs &a, hipStream_t stream)
 //     233                       156, 145             169, 147             172, 181
 //     273, evenly               170, 156             180, 154             150, not timed
 //     930                       394, 440             412, 424             583, 576
+// (The rule does not follow every line: 8 experts of 768 x 2048 at 1024 rows go forward in tiles of 256, 42 us against 38.)
 template <int DT, int FORM, bool GATHER>
 hipError_t pick(const ProductArgs &a, hipStream_t stream)
 {

@@ -720,7 +720,9 @@ def expert_product_forward(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPl
 
     ``weight`` [experts, out, in]; ``x`` [slots, in] in the plan's order, or with ``gather`` the tokens
     [..., in] whose choices the plan sorted, each read wherever one of its slots stands.  Rows of no expert are 0.
-    bfloat16 or float16, in and out multiples of 8; sums are fp32, rounded once."""
+    bfloat16 or float16, in and out multiples of 8; sums are fp32, rounded once.  Rows of ``x`` and ``weight`` are read where they
+    lie if they are dense and begin on 16 bytes; otherwise the whole tensor is copied first, in each call and in the backward
+    pass again (so is a weight kept as [experts, in, out] and passed transposed)."""
     keep, head = _product_args(x, weight, plan, gather)
     y = torch.empty((plan.rows.numel(), weight.shape[1]), dtype=x.dtype, device=x.device)
     _call(x.device, lm_lib().stq_expert_product_forward, _PRODUCT.pack(*head, y.data_ptr(), *(0,) * 7))
@@ -730,7 +732,8 @@ def expert_product_forward(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPl
 def expert_product_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *, gather: bool = False,
                             inputs: bool = True, weights: bool = True, dtype: Optional[torch.dtype] = None):
     """``(dx, dweight)``: the gradients of ``x`` (with ``gather`` summed over a token's slots in fp32) and of ``weight``, in
-    ``dtype`` (its own type or float32); None for what ``inputs`` or ``weights`` leaves out.  An expert without rows gets zeros."""
+    ``dtype`` (its own type or float32; autograd takes its own); None for what ``inputs`` or ``weights`` leaves out.  An
+    expert without rows gets zeros."""
     keep, head = _product_args(x, weight, plan, gather)
     want = (plan.rows.numel(), weight.shape[1])
     if dy.shape != want or dy.dtype != x.dtype:
@@ -897,8 +900,9 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, norm: Optional
     a synchronisation.
 
     ``grads``: dense fp32, bf16 or fp16 tensors of one device, apart from each other in memory (a parameter without a gradient
-    is left out).  ``out``: tensors like them that take the result in their place.  ``norm``: a fp32 scalar to scale by, e.g. one formed over several ranks.
-    A norm of NaN makes every gradient NaN, an infinite one 0 (its infinite ones NaN)."""
+    is left out).  ``out``: tensors like them that take the result in their place.  ``norm``: a fp32 scalar to scale by,
+    e.g. one formed over several ranks.  Long lists cost the host about 1 us a tensor; thousands of tensors also cost the device more
+    than their bytes.  A norm of NaN makes every gradient NaN, an infinite one 0 (its infinite ones NaN)."""
     grads, into, packed = _grad_list(grads, out)
     if not grads:
         _fail("no gradients")
