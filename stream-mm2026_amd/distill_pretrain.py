@@ -41,8 +41,8 @@ class Decoder(torch.nn.Module):
     """A decoder with norms before and after each attention and MLP block (GPT-2 small's sizes by default)."""
 
     def __init__(self, vocab: int = VOCAB, n_embd: int = 768, n_layer: int = 12, n_head: int = 12, n_kv: int = 0,
-                 window: int = 0, sinks: int = 0, experts: int = 0, top_experts: int = 2, expert_width: int = 0, seed: int = 42,
-                 device="cuda:0"):
+                 window: int = 0, sinks: int = 0, seed: int = 42, device="cuda:0", *, experts: int = 0, top_experts: int = 2,
+                 expert_width: int = 0):
         super().__init__()
         g = torch.Generator().manual_seed(seed)
         self.experts, self.top_experts = experts, top_experts
