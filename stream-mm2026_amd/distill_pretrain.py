@@ -39,6 +39,7 @@ from gpt2_pretrain import OPTIMIZERS, VOCAB, build_optimizer  # noqa: E402
 
 class Decoder(torch.nn.Module):
     """A decoder with norms before and after each attention and MLP block (GPT-2 small's sizes by default)."""
+    experts, uneven = 0, None            # (a dense one)
 
     def __init__(self, vocab: int = VOCAB, n_embd: int = 768, n_layer: int = 12, n_head: int = 12, n_kv: int = 0,
                  window: int = 0, sinks: int = 0, seed: int = 42, device="cuda:0", *, experts: int = 0, top_experts: int = 2,
@@ -121,18 +122,20 @@ def teach(teacher: Decoder, tokens: torch.Tensor, k: int):
 
 def step_loss(model: Decoder, tokens: torch.Tensor, targets, *, temperature: float, alpha: float, balance: float = 0.01) -> torch.Tensor:
     """Forward and backward of one batch: the mean loss; the gradients are in the parameters, with ``balance`` times
-    those of how unevenly experts are loaded."""
+    those of how unevenly experts are loaded, where the model (or the ``module`` that it wraps) says so."""
     logits = model(tokens)
     labels = torch.full_like(tokens, -100)
     labels[:, :-1] = tokens[:, 1:]
     # the gradient takes the logits' place: nothing else needs them
     z = logits.detach()
     loss, dz = lm.distill_loss_and_grad(z, *targets, grad=1.0 / tokens.numel(), labels=labels, temperature=temperature, alpha=alpha, out=z)
-    if model.uneven is None:
+    inner = model if hasattr(model, "uneven") else getattr(model, "module", model)      # (as wrappers for several ranks hold it)
+    uneven = getattr(inner, "uneven", None)
+    if uneven is None:
         logits.backward(dz)
     else:
-        torch.autograd.backward([logits, balance * model.uneven], [dz, None])
-        model.uneven = model.uneven.detach()         # (the number: its graph would live until the next call)
+        torch.autograd.backward([logits, balance * uneven], [dz, None])
+        inner.uneven = uneven.detach()         # (the number: its graph would live until the next call)
     return loss.mean()
 
 
