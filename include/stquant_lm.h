@@ -266,7 +266,7 @@ int stq_expert_combine_backward(const stq_expert_combine *a, void *stream);
 
 /*
  * The 2-norm of all tensors together, and out = grad min(1, max_norm / (norm + 1e-6)), of which a NaN norm makes NaN and
- * an infinite one 0 (NaN where the gradient is infinite).  Squares are added in double.  norm: one float on the
+ * an infinite one 0 (NaN where the gradient is infinite, or max_norm).  Squares are added in double.  norm: one float on the
  * device.  given (or null): a norm to scale by in place of theirs, e.g. one summed over ranks; norm is then not written.
  * out may be grad; otherwise it lies apart from every grad and out of the list.  numel up to 2^36,
  * count to 2^24.  workspace: stq_clip_workspace(a) bytes (from count alone), 16-byte aligned.  The list is read before the call returns.

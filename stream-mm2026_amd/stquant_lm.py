@@ -902,7 +902,8 @@ def clip_grads(grads: Iterable[torch.Tensor], max_norm: float, *, norm: Optional
     ``grads``: dense fp32, bf16 or fp16 tensors of one device, apart from each other in memory (a parameter without a gradient
     is left out).  ``out``: tensors like them that take the result in their place.  ``norm``: a fp32 scalar to scale by,
     e.g. one formed over several ranks.  Long lists cost the host about 1 us a tensor; thousands of tensors also cost the device more
-    than their bytes.  A norm of NaN makes every gradient NaN, an infinite one 0 (its infinite ones NaN)."""
+    than their bytes.  A norm of NaN makes every gradient NaN, an infinite one 0 (its infinite ones NaN; with an infinite
+    ``max_norm``, which otherwise leaves them alone, all NaN)."""
     grads, into, packed = _grad_list(grads, out)
     if not grads:
         _fail("no gradients")

@@ -123,6 +123,15 @@ def test_nan_and_infinity():
             assert bool(torch.isnan(grads[0]).all()) and bool(torch.isnan(grads[1]).all())
 
 
+def test_an_infinite_limit():
+    """It leaves the bits alone, and of an infinite norm makes inf / inf."""
+    g = tensors([500, 33], BF16)
+    before = [t.clone() for t in g]
+    assert float(lm.clip_grads(g, float("inf"))) == float(lm.grad_norm(before)) and all(torch.equal(a, b) for a, b in zip(g, before))
+    g[0][3] = float("inf")
+    assert float(lm.clip_grads(g, float("inf"))) == float("inf") and bool(torch.isnan(g[0]).all()) and bool(torch.isnan(g[1]).all())
+
+
 def test_zero_norms_and_limits():
     z = [torch.zeros(500, device="cuda")]
     assert float(lm.clip_grads(z, 1.0)) == 0.0 and not bool(z[0].any())
