@@ -7,8 +7,8 @@
 // be captured).  Memory bound: the gradients are read twice, as their norm must be known before the first is written: GPT-2
 // small's in fp32 95 us for the norm (5.2 TB/s) and 176 for the scaling (5.7), 1.88 G elements of bf16 680 (5.5) and 1444 (5.2).
 // Results are stored past the caches.  What follows decides little: with the gradients written before and the 4-bit optimizer's
-// step behind, clipping adds 268-270 us to GPT-2 small's, 97-103 to 30 M parameters and 63 to 2.4 M, with ordinary stores 270-272,
-// 99 and 65.  (In a loop of clippings alone, written-back results slow the next norm: 129 us.)
+// step behind, clipping adds 268-270 us to GPT-2 small's, 91-103 to 30 M parameters and 54-64 to 2.4 M, with ordinary stores 270-272,
+// 98-101 and 63-67.  (In a loop of clippings alone, written-back results slow the next norm: 129 us.)
 // Every workgroup of the scaling adds up the norm's partial sums for itself, up to 2048 doubles for each launch of the norm: 1.13 G
 // elements of bf16 take 1260 us as 160 or 320 tensors, 1310 as 1080, 1590 as 2160 and 2680 as 4320 (the host's side of such a
 // list is 4800).
